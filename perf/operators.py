@@ -165,7 +165,8 @@ def _quantized(x):
     """x [pages, kv, D, 16] to e4m3 and one power of two for each page and
     head: the least of those whose multiple of 448 holds all of it."""
     m, e = torch.frexp(x.abs().amax((2, 3)))
-    scale = torch.exp2(torch.clamp(e - 9 + (m > 0.875), min=-126).float())
+    e = torch.where(m > 0, e - 9 + (m > 0.875), -126)
+    scale = torch.exp2(e.clamp(min=-126).float())
     return (x / scale[..., None, None]).to(E4M3), scale
 
 
@@ -297,7 +298,8 @@ def _write(state):
             0, page[:, None].expand(-1, x.shape[1]),
             x.nan_to_num(0.0).abs().amax(-1), "amax")
         m, e = torch.frexp(big[page])
-        fit = torch.exp2((e - 9 + (m > 0.875)).clamp(min=-126).float())
+        e = torch.where(m > 0, e - 9 + (m > 0.875), -126)
+        fit = torch.exp2(e.clamp(min=-126).float())
         was = scales[page, :, i]
         now = torch.where(keep[:, None], torch.maximum(was, fit), fit)
         raw = cache.view(torch.uint8)
