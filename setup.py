@@ -46,6 +46,10 @@ ext_modules = [
                 "linear.hip",
                 "skinny_gemm.hip",
                 "packed_gemm.hip",
+                "kv8_bindings.cpp",
+                "kv8_cache.hip",
+                "kv8_decode.hip",
+                "kv8_prefill.hip",
             )
         ],
         extra_compile_args={

@@ -1,0 +1,477 @@
+"""The kernels of a paged cache held in 8 bits against its definition in 64 bits.
+
+What pages hold is compared for equality: scales are powers of two, a value times one
+is exact, and one rounding to e4m3 is left. Attention: results are bf16, off by up to
+2^-8 of themselves. Its scores are sums of D exact products in 32 bits, off by up to
+2^-24 D of the sum of their sizes, and what the exponent is made of by 2^-22 more: a
+weight is off by as much of itself, numerator and denominator. Weights of decoded rows
+have two truncated bf16 terms, off by 2^-15 of themselves; those of prompts are
+rounded to bf16, 2^-8."""
+import math
+
+import pytest
+import torch
+
+from xllm_service_amd import ops
+
+from kv8_oracle import Cache, attend, layout, same, slots_of
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def rows(T, heads, dim, seed, big=1.0, beside=2):
+    """bf16 rows in the middle of wider ones, on the CPU."""
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(T, (heads + beside) * dim, generator=g) * big)
+    return x.to(torch.bfloat16)
+
+
+def part(x, heads, dim):
+    """Their heads, on the GPU, as a view of the wider rows."""
+    return x.to(DEV)[:, dim:(1 + heads) * dim].unflatten(1, (heads, dim))
+
+
+def ints(x, dtype=torch.int32):
+    return torch.tensor(x, dtype=dtype, device=DEV)
+
+
+def filled(lens, heads, dim, seed, spare=3, big=1.0):
+    """A cache of these sequences, written by the reference on the CPU, every other
+    byte of it NaN and other scales 2^60: (cache on the GPU, oracle, table)."""
+    table, pages = layout(lens, spare, seed)
+    cache = ops.kv8_cache(pages, heads, dim)
+    slots = slots_of(table, [0] * len(lens), [max(n, 0) for n in lens])
+    g = torch.Generator().manual_seed(seed)
+    k, v = (torch.randn(len(slots), heads, dim, generator=g) * big
+            for _ in range(2))
+    k = k.to(torch.bfloat16)
+    v = (v * torch.exp2(torch.randn(heads, 1, generator=g))).to(torch.bfloat16)
+    ops.reshape_and_cache_kv8(k, v, *cache, torch.tensor(slots).long())
+    want = Cache(pages, heads, dim).load(*cache)
+    live = torch.zeros(pages * 16, dtype=torch.bool)
+    live[slots] = True
+    live = live.view(pages, 16)
+    kb, vb = (c.view(torch.uint8) for c in cache[:2])
+    kb.transpose(2, 3).transpose(1, 2)[~live] = 0x7f
+    vb.permute(0, 3, 1, 2)[~live] = 0x7f
+    cache[2][~live.any(1)] = 2.0 ** 60
+    return tuple(c.to(DEV) for c in cache), want, table
+
+
+def close(got, q, want, table, cu, total, scale, weights):
+    k, v = want.values(0), want.values(1)
+    ref, big, most = attend(q, k, v, table, cu, total, scale)
+    off = 2.0 ** -24 * q.shape[2] * most + 2.0 ** -22 * most.clamp(min=1.0)
+    bound = 2.0 ** -8 * ref.abs() + (weights + 2 * off) * big + 1e-30
+    diff = (got.cpu().double() - ref).abs()
+    assert not diff.isnan().any()
+    assert (diff <= bound).all(), float((diff / bound).max())
+
+
+# ---- writing -----------------------------------------------------------------
+@pytest.mark.parametrize("heads,dim", [(1, 64), (3, 128), (8, 128), (12, 64)])
+def test_write(heads, dim):
+    pages = 7
+    cache = tuple(c.to(DEV) for c in ops.kv8_cache(pages, heads, dim))
+    want = Cache(pages, heads, dim)
+    steps = [list(range(16, 16 + 21)), [37], [38, 39], [40, -1, 41, 0],
+             [1, 10 ** 9, -7, 112], [2, 2], [17, 17, 16, 19, 17],
+             list(range(48, 64)) + list(range(95, 79, -1)),
+             [9, 60, 100, 90, 30]]
+    for n, slots in enumerate(steps):
+        k, v = (rows(len(slots), heads, dim, 2 * n + i, 2.5 ** (n % 5 - 2))
+                for i in range(2))
+        gk, gv = part(k, heads, dim), part(v, heads, dim)
+        ops.reshape_and_cache_kv8(gk, gv, *cache, ints(slots, torch.long))
+        want.write(gk, gv, slots)
+        got = Cache(pages, heads, dim).load(*cache)
+        for i in range(2):
+            assert same(got.x[i], want.x[i]), (n, i)
+        assert same(got.scale, want.scale), n
+
+
+def test_write_again_over_far_scales():
+    """A page that goes on: from nothing, from NaN bytes, past what one power of
+    two of fp32 spans, without growing, and with zeros."""
+    cache = tuple(c.to(DEV) for c in ops.kv8_cache(2, 1, 64))
+    want = Cache(2, 1, 64)
+    for slot, big in ((3, 0.0), (4, 1e-38), (5, 1e-30), (6, 3e38), (7, 1.0),
+                      (8, math.inf), (9, math.nan), (10, 0.0), (16, math.inf),
+                      (17, -0.0)):
+        x = torch.full((1, 1, 64), big).to(torch.bfloat16)
+        x[0, 0, ::3] *= -0.5
+        x = x.to(DEV)
+        ops.reshape_and_cache_kv8(x, x, *cache, ints([slot], torch.long))
+        want.write(x, x, [slot])
+        got = Cache(2, 1, 64).load(*cache)
+        for i in range(2):
+            assert same(got.x[i], want.x[i]), slot
+        assert same(got.scale, want.scale), slot
+
+
+@pytest.mark.parametrize("offset", [0, 1, 8])
+def test_write_rows_at_any_address(offset):
+    """Keys are read by 16 B: rows that are not aligned are copied."""
+    cache = tuple(c.to(DEV) for c in ops.kv8_cache(3, 2, 128))
+    want = Cache(3, 2, 128)
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(20, 2 * 128 + 9, generator=g).to(torch.bfloat16).to(DEV)
+    k = x[:, offset:offset + 256].unflatten(1, (2, 128))
+    v = x[:, 9 - offset:265 - offset].unflatten(1, (2, 128))
+    slots = list(range(5, 25))
+    ops.reshape_and_cache_kv8(k, v, *cache, ints(slots, torch.long))
+    want.write(k, v, slots)
+    got = Cache(3, 2, 128).load(*cache)
+    assert all(same(got.x[i], want.x[i]) for i in range(2))
+
+
+# ---- tables ------------------------------------------------------------------
+@pytest.mark.parametrize("seqs,most_old,most_new,short", [
+    (1, 0, 1, 0), (1, 100, 3, 0), (3, 40, 40, 0), (256, 300, 2, 0),
+    (257, 300, 1, 0), (700, 90, 60, 0), (64, 2000, 1500, 0), (50, 60, 60, 9)])
+def test_tables_from_lengths(seqs, most_old, most_new, short):
+    g = torch.Generator().manual_seed(seqs)
+    old = torch.randint(0, most_old + 1, (seqs,), generator=g).int()
+    new = old + torch.randint(-2, most_new + 1, (seqs,), generator=g).int()
+    width = (int(new.max()) + 47) // 16 - short // 4
+    # rows of a wider table
+    table = torch.randint(0, 10 ** 6, (seqs, width + 3), generator=g).int()
+    pages = int(((new.clamp(min=0) + 15) // 16).sum())
+    free = torch.randperm(pages + 5, generator=g).int()[short * 9:]
+    room = int((new - old).clamp(min=0).sum()) + 7 - 11 * short
+    there = table.to(DEV)
+    got = ops.extend_block_tables(there[:, :width], old.to(DEV), new.to(DEV),
+                                  free.to(DEV), room)
+    want = ops.extend_block_tables(table[:, :width], old, new, free, room)
+    assert torch.equal(there.cpu(), table)
+    for a, b in zip(got, want):
+        assert torch.equal(a.cpu(), b)
+
+
+# ---- attention ---------------------------------------------------------------
+SHAPES = [(2, 4, 128), (1, 7, 128), (3, 1, 64), (2, 16, 128), (2, 12, 64),
+          (1, 1, 128)]
+
+
+@pytest.mark.parametrize("heads,per,dim", SHAPES)
+@pytest.mark.parametrize("lens", [
+    [1], [0, 1, 15, 16, 17, 31, 32, 33, 47, 48, 49, 64, 65], [300, 0, 129],
+    [1500], [700, 3000, 5, 1029]], ids=lambda x: f"{len(x)}x{max(x)}")
+def test_decode(heads, per, dim, lens):
+    cache, want, table = filled(lens, heads, dim, len(lens))
+    H, S = heads * per, len(lens)
+    q = part(rows(S, H, dim, 5), H, dim)
+    out = torch.full((S, H + 1, dim), 7.0, dtype=torch.bfloat16, device=DEV)
+    ops.paged_attn_decode_kv8(q, *cache, table.to(DEV), ints(lens),
+                              dim ** -0.5, out=out[:, :H])
+    close(out[:, :H], q, want, table, list(range(S + 1)), lens, dim ** -0.5,
+          2.0 ** -15)
+    assert (out[:, H] == 7.0).all()
+    plain = ops.paged_attn_decode_kv8(q, *cache, table.to(DEV), ints(lens),
+                                      dim ** -0.5)
+    assert torch.equal(plain, out[:, :H])
+
+
+@pytest.mark.parametrize("seqs", [40, 90, 140])
+def test_decode_many(seqs):
+    """Sequences that fill the card once and more, lengths far apart."""
+    lens = [(37 * i) % 601 for i in range(seqs)]
+    cache, want, table = filled(lens, 2, 128, seqs)
+    q = part(rows(seqs, 8, 128, 5), 8, 128)
+    got = ops.paged_attn_decode_kv8(q, *cache, table.to(DEV), ints(lens), 0.09)
+    close(got, q, want, table, list(range(seqs + 1)), lens, 0.09, 2.0 ** -15)
+
+
+@pytest.mark.parametrize("heads,per,dim", SHAPES)
+@pytest.mark.parametrize("new,old", [
+    ([1], [0]), ([3, 1, 16, 0, 33], [0, 31, 16, 9, 0]), ([64, 65], [63, 0]),
+    ([130], [0]), ([200], [1100]), ([70, 1, 300], [1000, 1200, 0]),
+    ([17] * 70, [5] * 70)], ids=lambda x: f"{len(x)}x{max(x)}")
+def test_prefill(heads, per, dim, new, old):
+    lens = [n + o for n, o in zip(new, old)]
+    cache, want, table = filled(lens, heads, dim, len(lens))
+    H, T = heads * per, sum(new)
+    q = part(rows(T + 3, H, dim, 6), H, dim)
+    cu = [sum(new[:i]) for i in range(len(new) + 1)]
+    out = torch.full((T + 3, H + 1, dim), 7.0, dtype=torch.bfloat16, device=DEV)
+    ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints(cu), ints(lens),
+                               dim ** -0.5, out=out[:, :H])
+    close(out[:T, :H], q[:T], want, table, cu, lens, dim ** -0.5, 2.0 ** -8)
+    assert (out[T:] == 7.0).all() and (out[:, H] == 7.0).all()
+
+
+@pytest.mark.parametrize("heads,per,dim", [(8, 4, 128), (4, 7, 128), (12, 1, 64)])
+@pytest.mark.parametrize("new,old", [
+    ([1300], [0]), ([600, 900, 40], [700, 0, 2000]), ([400] * 5, [100] * 5)],
+    ids=lambda x: f"{len(x)}x{max(x)}")
+def test_prefill_of_full_steps(heads, per, dim, new, old):
+    lens = [n + o for n, o in zip(new, old)]
+    cache, want, table = filled(lens, heads, dim, len(lens), big=2.0)
+    H, T = heads * per, sum(new)
+    q = part(rows(T, H, dim, 6), H, dim)
+    cu = [sum(new[:i]) for i in range(len(new) + 1)]
+    got = ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints(cu),
+                                     ints(lens), dim ** -0.5)
+    close(got, q, want, table, cu, lens, dim ** -0.5, 2.0 ** -8)
+
+
+def test_rows_without_keys():
+    """Lengths of zero and below, chunks longer than their sequence, tables without
+    columns."""
+    cache, want, table = filled([20, 30], 2, 128, 1)
+    q = part(rows(12, 4, 128, 2), 4, 128)
+    tab = table.to(DEV)
+    cu, total = [0, 5, 12], [2, -3]
+    got = ops.paged_attn_prefill_kv8(q, *cache, tab, ints(cu), ints(total), 0.1)
+    assert (got[:3] == 0).all() and (got[5:] == 0).all()
+    close(got, q, want, table, cu, total, 0.1, 2.0 ** -8)
+    got = ops.paged_attn_decode_kv8(q[:2], *cache, tab, ints([0, -100]), 0.1)
+    assert (got == 0).all()
+    none = tab[:, :0].contiguous()
+    got = ops.paged_attn_decode_kv8(q[:2], *cache, none, ints([5, 9]), 0.1)
+    assert (got == 0).all()
+    got = ops.paged_attn_prefill_kv8(q, *cache, none, ints(cu), ints([5, 9]), 0.1)
+    assert (got == 0).all()
+
+
+def test_tables_that_end_before_their_sequence():
+    """Keys behind a table's end are not there; entries of no page are page 0."""
+    lens = [40, 25]
+    cache, want, table = filled(lens, 2, 64, 4)
+    table[1, 1] = table[0, 0]
+    wild = table.clone()
+    table[table == table[0, 1]] = 0
+    wild[wild == wild[0, 1]] = 10 ** 6
+    wild[1, 2] = -5
+    q = part(rows(9, 4, 64, 2), 4, 64)
+    total = [100, 25]
+    got = ops.paged_attn_decode_kv8(q[:2], *cache, wild.to(DEV), ints(total), 0.1)
+    ok = want.values(1)[table[0, 2]][:, 8:].isnan()      # none of the oracle's
+    assert not ok.any()
+    # page 0 and what the last page holds behind 40 tokens: finite ones here
+    for c in cache[:2]:
+        c.view(torch.uint8)[c.view(torch.uint8) == 0x7f] = 0
+    cache[2][cache[2] == 2.0 ** 60] = 1.0
+    want.load(*cache)
+    got = ops.paged_attn_decode_kv8(q[:2], *cache, wild.to(DEV), ints(total), 0.1)
+    close(got, q[:2], want, table, [0, 1, 2], total, 0.1, 2.0 ** -15)
+    got = ops.paged_attn_prefill_kv8(q, *cache, wild.to(DEV), ints([0, 4, 9]),
+                                     ints(total), 0.1)
+    close(got, q, want, table, [0, 4, 9], total, 0.1, 2.0 ** -8)
+
+
+def test_negative_scales_and_large_scores():
+    lens = [50, 333]
+    cache, want, table = filled(lens, 2, 128, 7, big=30.0)
+    q = part(rows(2, 8, 128, 2, 9.0), 8, 128)
+    for scale in (-0.3, 0.0, 2.0):
+        got = ops.paged_attn_decode_kv8(q, *cache, table.to(DEV), ints(lens),
+                                        scale)
+        close(got, q, want, table, [0, 1, 2], lens, scale, 2.0 ** -15)
+        got = ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV),
+                                         ints([0, 1, 2]), ints(lens), scale)
+        close(got, q, want, table, [0, 1, 2], lens, scale, 2.0 ** -8)
+
+
+def test_values_that_are_not_finite():
+    """A NaN among a sequence's keys or values is seen by the rows that see it, and
+    by no others."""
+    lens = [40, 70]
+    cache, want, table = filled(lens, 1, 64, 8)
+    cache[1].view(torch.uint8)[table[1, 1], 0, 5, 4] = 0x7f      # token 20
+    q = part(rows(110, 2, 64, 3), 2, 64)
+    got = ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints([0, 40, 110]),
+                                     ints(lens), 0.1).cpu()
+    assert not got[:60].isnan().any()
+    assert got[60:, :, 5].isnan().all()
+    assert not got[60:, :, :5].isnan().any()
+    got = ops.paged_attn_decode_kv8(q[:2], *cache, table.to(DEV), ints([40, 20]),
+                                    0.1)
+    assert not got.isnan().any()
+    got = ops.paged_attn_decode_kv8(q[:2], *cache, table.to(DEV), ints([40, 21]),
+                                    0.1).cpu()
+    assert got[1, :, 5].isnan().all() and not got[0].isnan().any()
+
+
+def test_pages_past_32_bits():
+    """A pool of over 4 GiB of keys: its last pages are written and read."""
+    heads, dim, pages = 8, 128, 270000
+    cache = ops.kv8_cache(pages, heads, dim, DEV)
+    table = torch.tensor([[pages - 1, 3, pages - 7, 262145]]).int()
+    slots = slots_of(table, [0], [60])
+    k, v = rows(60, heads, dim, 1), rows(60, heads, dim, 2)
+    gk, gv = part(k, heads, dim), part(v, heads, dim)
+    ops.reshape_and_cache_kv8(gk, gv, *cache, ints(slots, torch.long))
+    want = Cache(4, heads, dim)
+    want.write(gk, gv, list(range(60)))
+    got = Cache(4, heads, dim).load(
+        *(c.view(torch.uint8)[table[0].long().to(DEV)].view(c.dtype)
+          if c.dtype == torch.float8_e4m3fn else c[table[0].long().to(DEV)]
+          for c in cache))
+    assert all(same(got.x[i], want.x[i]) for i in range(2))
+    q = part(rows(60, 32, dim, 3), 32, dim)
+    tab, near = table.to(DEV), torch.arange(4).int()[None]
+    out = ops.paged_attn_prefill_kv8(q, *cache, tab, ints([0, 60]), ints([60]),
+                                     0.1)
+    close(out, q, want, near, [0, 60], [60], 0.1, 2.0 ** -8)
+    out = ops.paged_attn_decode_kv8(q[:1], *cache, tab, ints([60]), 0.1)
+    close(out, q[:1], want, near, [0, 1], [60], 0.1, 2.0 ** -15)
+
+
+def test_long_sequence():
+    lens = [40000, 33]
+    cache, want, table = filled(lens, 1, 64, 9)
+    q = part(rows(2, 4, 64, 3), 4, 64)
+    got = ops.paged_attn_decode_kv8(q, *cache, table.to(DEV), ints(lens), 0.2)
+    close(got, q, want, table, [0, 1, 2], lens, 0.2, 2.0 ** -15)
+
+
+# ---- together, streams and graphs ----------------------------------------------
+def step(cache, table, lens, new, free, k, v, q, out):
+    slots, _, cu, used = ops.extend_block_tables(table, lens, new, free,
+                                                 k.shape[0])
+    ops.reshape_and_cache_kv8(k, v, *cache, slots)
+    ops.paged_attn_prefill_kv8(q, *cache, table, cu, new, 0.1, out=out)
+    return slots, cu, used
+
+
+def test_a_run_of_them():
+    heads, per, dim, S = 2, 4, 128, 3
+    table = torch.zeros(S, 20, dtype=torch.int32, device=DEV)
+    free = torch.randperm(64, generator=torch.Generator().manual_seed(1))
+    free = free.int().to(DEV)
+    cache = ops.kv8_cache(64, heads, dim, DEV)
+    want = Cache(64, heads, dim)
+    lens, at = torch.zeros(S, dtype=torch.int32, device=DEV), 0
+    for n, grow in enumerate(([100, 0, 17], [1, 1, 1], [0, 130, 1], [1, 1, 14],
+                              [1, 1, 1])):
+        T = sum(grow)
+        k, v, q = (part(rows(T, m, dim, 3 * n + i), m, dim) for i, m in
+                   enumerate((heads, heads, heads * per)))
+        out = torch.empty(q.shape, dtype=q.dtype, device=DEV)
+        new = lens + ints(grow)
+        slots, cu, used = step(cache, table, lens, new, free[at:], k, v, q, out)
+        at += int(used)
+        want.write(k, v, slots.tolist())
+        close(out, q, want, table.cpu(), cu.tolist(), new.tolist(), 0.1,
+              2.0 ** -8)
+        if max(grow) == min(grow) == 1:
+            one = ops.paged_attn_decode_kv8(q, *cache, table, new, 0.1)
+            close(one, q, want, table.cpu(), cu.tolist(), new.tolist(), 0.1,
+                  2.0 ** -15)
+        lens = new
+
+
+def test_captured_steps():
+    """Two captured steps that share a pool, replayed by turns with eager work
+    between them: each replay is the eager result. Rows of padding have no slot."""
+    heads, per, dim, S = 2, 4, 128, 4
+    lens0 = [700, 3000, 30, 0]
+    cache, _, table = filled([n + 64 for n in lens0], heads, dim, 3, spare=9)
+    spare = sorted(set(range(cache[2].shape[0])) - set(table.flatten().tolist()))
+    table = table.to(DEV)
+    free, grow = ints(spare[:3]), ints([1, 1, 1, 0])
+    x = part(rows(S, 2 * heads + heads * per, dim, 1), 2 * heads + heads * per,
+             dim)
+
+    def run(lens, x):
+        new = lens + grow
+        slots, *_ = ops.extend_block_tables(table, lens, new, free, S)
+        ops.reshape_and_cache_kv8(x[:, :heads], x[:, heads:2 * heads], *cache,
+                                  slots)
+        return ops.paged_attn_decode_kv8(x[:, 2 * heads:], *cache, table, new,
+                                         0.1)
+    graphs, pool = [], None
+    for g in range(2):
+        lens, xx = ints(lens0), x.clone()
+        run(lens, xx)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            out = run(lens, xx)
+        pool = graph.pool()
+        graphs.append((graph, lens, xx, out))
+    for n in range(6):
+        graph, lens, xx, out = graphs[n % 2]
+        lens.copy_(ints([k + n for k in lens0[:3]] + [0]))
+        xx.copy_(x * (1 + n))
+        free.copy_(ints(spare[n:n + 3]))         # a page of its own for each
+        keep = [c.clone() for c in cache]
+        graph.replay()
+        torch.cuda.synchronize()
+        got, after = out.clone(), [c.clone() for c in cache]
+        for c, was in zip(cache, keep):
+            c.copy_(was)
+        want = run(lens.clone(), xx.clone())
+        assert torch.equal(got, want), n
+        for c, b in zip(cache, after):
+            assert torch.equal(c.view(torch.uint8), b.view(torch.uint8)), n
+        assert (got[3] == 0).all()
+
+
+def test_two_streams_at_once():
+    lens = [900, 2500, 64]
+    cache, want, table = filled(lens, 2, 128, 5)
+    tab, n = table.to(DEV), ints(lens)
+    q = [part(rows(3, 8, 128, i), 8, 128) for i in range(2)]
+    alone = [ops.paged_attn_decode_kv8(x, *cache, tab, n, 0.1) for x in q]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(ops.paged_attn_decode_kv8(q[i], *cache, tab, n,
+                                                         0.1))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, alone[i]) for o in outs[i])
+
+
+def test_refusals():
+    k8, v8, s = ops.kv8_cache(3, 2, 64, DEV)
+    x = torch.zeros(4, 2, 64, dtype=torch.bfloat16, device=DEV)
+    at = torch.zeros(4, dtype=torch.long, device=DEV)
+    tab, lens = ints([[0]] * 4), ints([1] * 4)
+    cu = ints([0, 4])
+
+    def no(f, *args, **kw):
+        with pytest.raises(RuntimeError):
+            f(*args, **kw)
+    w = ops.reshape_and_cache_kv8
+    no(w, x, x, k8, v8, s, at[:3])
+    no(w, x, x[:3], k8, v8, s, at)
+    no(w, x[:, :1], x, k8, v8, s, at)
+    no(w, x, x, k8, v8, s, at.int())
+    no(w, x, x, k8, v8, s, at.cpu())
+    no(w, x.float(), x, k8, v8, s, at)
+    no(w, x, x, k8.view(torch.uint8), v8, s, at)
+    no(w, x, x, k8.cpu(), v8, s, at)
+    no(w, x, x, k8, v8, s.double(), at)
+    no(w, x, x, k8[:2], v8, s, at)
+    no(w, x, x, v8, k8, s, at)
+    no(w, x, x, k8[:0], v8[:0], s[:0], at)
+    no(w, x.transpose(0, 1).contiguous().transpose(0, 1), x, k8, v8, s, at)
+    d, p = ops.paged_attn_decode_kv8, ops.paged_attn_prefill_kv8
+    no(d, x[:, :1], k8, v8, s, tab, lens, 1.0)
+    no(d, x[..., :32], k8, v8, s, tab, lens, 1.0)
+    no(d, x.half(), k8, v8, s, tab, lens, 1.0)
+    no(d, x, k8, v8, s, tab.long(), lens, 1.0)
+    no(d, x, k8, v8, s, tab[:3], lens, 1.0)
+    no(d, x, k8, v8, s, tab, lens[:3], 1.0)
+    no(d, x, k8, v8, s, tab, lens, 1.0, out=x[:3])
+    no(d, x, k8, v8, s, tab, lens, 1.0, out=x[:1].expand(4, 2, 64))
+    no(d, torch.zeros(4, 34, 64, dtype=x.dtype, device=DEV), k8, v8, s, tab, lens,
+       1.0)
+    no(p, x, k8, v8, s, tab, cu.long(), lens, 1.0)
+    no(p, x, k8, v8, s, tab, cu[:0], lens, 1.0)
+    no(p, x, k8, v8, s, tab[:0], cu, lens, 1.0)
+    no(p, x, k8, v8, s[:2], tab, cu, lens, 1.0)
+    e = ops.extend_block_tables
+    no(e, tab.long(), lens, lens, lens, 4)
+    no(e, tab, lens, lens[:2], lens, 4)
+    no(e, tab[:2], lens, lens, lens, 4)
+    no(e, tab, lens.cpu(), lens, lens, 4)
+    no(e, tab, lens, lens, lens, -1)
+    no(e, tab.expand(4, 3), lens, lens, lens, 4)

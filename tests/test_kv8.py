@@ -1,0 +1,182 @@
+"""A paged cache held in 8 bits: the references that run on a CPU, against the
+definition in 64 bits, and what they refuse."""
+import math
+
+import pytest
+import torch
+
+from xllm_service_amd import ops
+
+from kv8_oracle import Cache, attend, layout, same, slots_of
+
+
+def rows(T, heads, dim, seed, big=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(T, heads, dim, generator=g) * big
+    return x.to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_write_begins_goes_on_and_grows(dim):
+    cache = ops.kv8_cache(4, 2, dim)
+    want = Cache(4, 2, dim)
+    for step, slots in enumerate([
+            list(range(16, 16 + 21)),            # page 1 whole, page 2 begun
+            [37], [38], [39, 40],                # page 2 goes on
+            [-1, 41, -1, 4 * 16, 10 ** 9, -7],   # skipped: no slot of the cache
+            [0, 1], [2, 2],                      # two for one slot: the later
+            [16, 18]]):                          # page 1 anew, with a gap
+        # each step's are larger: scales grow over pages that go on
+        k, v = (rows(len(slots), 2, dim, 10 * step + i, 3.0 ** step)
+                for i in range(2))
+        ops.reshape_and_cache_kv8(k, v, *cache, torch.tensor(slots))
+        want.write(k, v, slots)
+        got = Cache(4, 2, dim).load(*cache)
+        for i in range(2):
+            assert same(got.x[i], want.x[i])
+        assert same(got.scale, want.scale)
+
+
+def test_scale_borders():
+    """Powers of two at the borders 448 * 2^e, zeros, and what is not finite."""
+    k = torch.zeros(16, 1, 64, dtype=torch.bfloat16)
+    v = k.clone()
+    for big, scale in ((448.0, 1.0), (450.0, 2.0), (224.0, 0.5), (0.0, 2.0 ** -126),
+                       (2.0 ** -133, 2.0 ** -126), (3.3e38, 2.0 ** 120)):
+        cache = ops.kv8_cache(1, 1, 64)
+        k[3, 0, 5], v[2, 0, 1] = big, -big
+        k[4, 0, 6], v[1, 0, 0] = math.inf, math.nan
+        ops.reshape_and_cache_kv8(k, v, *cache, torch.arange(16))
+        assert cache[2].tolist() == [[[scale, scale]]]
+        assert cache[0].float().isnan().sum() == 1
+        assert cache[1].float().isnan().sum() == 1
+
+
+@pytest.mark.parametrize("per", [1, 3])
+def test_attention_of_the_references(per):
+    lens, new, dim = [0, 1, 17, 40], [2, 1, 5, 40], 64
+    table, pages = layout(lens, 2, 1)
+    old = [0] * 4
+    cache = ops.kv8_cache(pages, 2, dim)
+    slots = slots_of(table, old, lens)
+    k, v = rows(len(slots), 2, dim, 2, 2.0), rows(len(slots), 2, dim, 3)
+    ops.reshape_and_cache_kv8(k, v, *cache, torch.tensor(slots))
+    ref = Cache(pages, 2, dim).load(*cache)
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    q = rows(cu[-1] + 2, 2 * per, dim, 4).float()
+    out = torch.full_like(q, 7.0)
+    ops.paged_attn_prefill_kv8(q, *cache, table, torch.tensor(cu).int(),
+                               torch.tensor(lens).int(), 0.125, out=out)
+    want, *_ = attend(q, ref.values(0), ref.values(1), table, cu, lens, 0.125)
+    assert torch.allclose(out[:-2].double(), want[:-2], atol=1e-5)
+    assert (out[-2:] == 7.0).all()               # behind the last sequence
+    assert (out[:2] == 0).all()                  # no keys
+    got = ops.paged_attn_decode_kv8(q[:4], *cache, table,
+                                    torch.tensor(lens).int(), 0.125)
+    want, *_ = attend(q[:4], ref.values(0), ref.values(1), table,
+                      list(range(5)), lens, 0.125)
+    assert torch.allclose(got.double(), want, atol=1e-5)
+
+
+def plan_of(table, old, new, free, room):
+    """Token by token, page by page."""
+    table = [list(map(int, r)) for r in table]
+    slots, pos, cu, at = [], [], [0], 0
+    for i, (a, b) in enumerate(zip(old, new)):
+        a = max(a, 0)
+        for p in range(a, max(b, a)):
+            if p % 16 == 0:
+                if at < len(free) and p // 16 < len(table[i]):
+                    table[i][p // 16] = free[at]
+                at += 1
+            first = -(-a // 16)
+            ok = p // 16 < len(table[i]) and (
+                p // 16 < first or at <= len(free))
+            slots.append(table[i][p // 16] * 16 + p % 16 if ok else -1)
+            pos.append(p)
+        cu.append(len(slots))
+    more = room - len(slots)
+    return table, (slots + [-1] * more)[:room], (pos + [0] * more)[:room], \
+        [min(c, room) for c in cu], [at]
+
+
+@pytest.mark.parametrize("old,new,free,width,room", [
+    ([0], [1], 1, 1, 1), ([15, 16, 17], [16, 17, 18], 5, 3, 3),
+    ([0, 5, 40, 3], [33, 5, 100, 2], 20, 8, 100),
+    ([7, 0], [7, 0], 3, 2, 4), ([], [], 2, 2, 3),
+    ([0, 0], [40, 40], 4, 3, 80),           # pages run out
+    ([0, 10], [50, 60], 9, 2, 200),         # tables too narrow
+    ([0, 3], [20, 20], 9, 4, 25),           # too little room
+    ([-3], [5], 2, 2, 5)])
+def test_tables_from_lengths(old, new, free, width, room):
+    g = torch.Generator().manual_seed(0)
+    table = torch.randint(100, 200, (len(old), width), generator=g).int()
+    ids = torch.randperm(50, generator=g)[:free].int()
+    want = plan_of(table, old, new, ids.tolist(), room)
+    got = ops.extend_block_tables(table, torch.tensor(old).int(),
+                                  torch.tensor(new).int(), ids, room)
+    assert table.tolist() == want[0]
+    assert [t.tolist() for t in got] == list(want[1:])
+    assert [t.dtype for t in got] == [torch.int64, torch.int64, torch.int32,
+                                      torch.int32]
+
+
+def test_a_run_of_them():
+    """Three steps of two sequences: planned, written and attended, against the
+    same over all tokens at once."""
+    table = torch.zeros(2, 4, dtype=torch.int32)
+    free = torch.tensor([5, 2, 7, 0, 3, 6, 1, 4]).int()
+    cache = ops.kv8_cache(8, 1, 64)
+    want = Cache(8, 1, 64)
+    lens, seed = torch.zeros(2, dtype=torch.int32), 0
+    for grow in ([20, 0], [1, 30], [1, 1]):
+        new = lens + torch.tensor(grow).int()
+        slots, pos, cu, used = ops.extend_block_tables(table, lens, new, free,
+                                                       sum(grow))
+        free = free[int(used):]
+        k, v, q = (rows(sum(grow), n, 64, seed + i) for i, n in
+                   enumerate((1, 1, 2)))
+        seed += 3
+        ops.reshape_and_cache_kv8(k, v, *cache, slots)
+        want.write(k, v, slots.tolist())
+        out = ops.paged_attn_prefill_kv8(q.float(), *cache, table, cu, new, 0.1)
+        ref, *_ = attend(q, want.values(0), want.values(1), table, cu.tolist(),
+                         new.tolist(), 0.1)
+        assert torch.allclose(out.double(), ref, atol=1e-5)
+        lens = new
+
+
+def test_refusals():
+    k8, v8, s = ops.kv8_cache(3, 2, 64)
+    x = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    at = torch.zeros(4, dtype=torch.long)
+    tab = torch.zeros(4, 1, dtype=torch.int32)
+    lens = torch.ones(4, dtype=torch.int32)
+
+    def no(f, *args):
+        with pytest.raises(RuntimeError):
+            f(*args)
+    no(ops.kv8_cache, 3, 2, 96)
+    w = ops.reshape_and_cache_kv8
+    no(w, x, x, k8, v8, s, at[:3])
+    no(w, x, x[:3], k8, v8, s, at)
+    no(w, x[:, :1], x, k8, v8, s, at)
+    no(w, x, x, k8, v8, s, at.int())
+    no(w, x, x, k8.view(torch.uint8), v8, s, at)
+    no(w, x, x, k8, v8, s.double(), at)
+    no(w, x, x, k8[:2], v8, s, at)
+    no(w, x, x, v8, k8, s, at)
+    d = ops.paged_attn_decode_kv8
+    no(d, x[:, :1], k8, v8, s, tab, lens, 1.0)
+    no(d, x[..., :32], k8, v8, s, tab, lens, 1.0)
+    no(d, x, k8, v8, s, tab.long(), lens, 1.0)
+    no(d, x, k8, v8, s, tab[:3], lens, 1.0)
+    no(d, x, k8, v8, s, tab, lens[:3], 1.0)
+    no(d, torch.zeros(4, 34, 64), k8, v8, s, tab, lens, 1.0)
+    cu = torch.tensor([0, 4]).int()
+    p = ops.paged_attn_prefill_kv8
+    no(p, x, k8, v8, s, tab, cu.long(), lens, 1.0)
+    no(p, x, k8, v8, s, tab[:0], cu, lens, 1.0)
+    no(p, x, k8, v8, s[:2], tab, cu, lens, 1.0)

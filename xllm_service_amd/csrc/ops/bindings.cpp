@@ -893,7 +893,10 @@ void enable_peer_access(long device, long peer) {
 
 }  // namespace
 
+void bind_kv8(pybind11::module& m);       // kv8_bindings.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  bind_kv8(m);
   m.def("rmsnorm", &rmsnorm);
   m.def("fused_add_rmsnorm", &fused_add_rmsnorm);
   m.def("rope", &rope);

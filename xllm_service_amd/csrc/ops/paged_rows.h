@@ -51,6 +51,7 @@
 #include <algorithm>
 #include <climits>
 
+#include "kv8.h"
 #include "paged_merge.h"
 
 namespace xllm {
@@ -345,7 +346,12 @@ XLLM_DEV bool pf_parts(int b, int least, int most, int groups, int turn,
 // KG: groups of four waves, each with the same rows and its share of the tiles: what
 // splitting keys over workgroups does, without partial results in memory.
 // SORT: the longest chains first, where keys are not split.
-template <int D, int TERMS, bool MORE, int KG, bool SPLIT, bool SORT = true>
+// CACHE8: pages of 8 bits (kv8.h). They take the way through registers, where a wave
+// converts its page to bf16 a step before its tile is multiplied: once for the 128 rows
+// that read it. Values come by channel, so their tile has channels for rows and keys for
+// columns, and an operand is one read of 16 B.
+template <int D, int TERMS, bool MORE, int KG, bool SPLIT, bool SORT = true,
+          bool CACHE8 = false>
 __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
     // (what the first loads need comes first: these are in registers)
     const int* __restrict__ block_tables,    // [num_seqs, max_blocks]
@@ -364,7 +370,7 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
     const PagedMeet meet,                    // [blocks]: its first part's counts
     const float scale, const long q_stride, const long out_stride,
     const int least, const int most, const int turn, const PagedMore x,
-    const PagedAhead ahead) {
+    const PagedAhead ahead, const Kv8Pages c8) {
   constexpr int KS = D / 16;                 // k steps of a score product
   constexpr int DT = D / 32;                 // 32-wide tiles of the head
   constexpr int CPR = D / 8;                 // 16 B chunks of a row
@@ -373,6 +379,7 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
   constexpr int TILE = PF_KT * D;            // elements of a K or V tile
   __shared__ __attribute__((aligned(1024))) unsigned short
       kv_lds[KG * 4 * TILE];
+  __shared__ int nan_lds[CACHE8 ? KG * 8 : 1];   // pages with a value that is none
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -408,10 +415,12 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
   const int ctx = seq_len - q_len;
   const int rows = q_len * G;
   const int n_qheads = n_kv * G;
+  // a table that ends before its sequence: what it does not have is not seen
+  const int room = CACHE8 ? max_blocks * PF_BS : INT_MAX;
 
   const int row0 = lt * PF_ROWS;
   const int kmax = ctx + pf_div(min(row0 + PF_ROWS, rows) - 1, by_G, sG) + 1;
-  const int n_tiles = (kmax + PF_KT - 1) / PF_KT;
+  const int n_tiles = (CACHE8 ? min(kmax, room) + PF_KT - 1 : kmax + PF_KT - 1) / PF_KT;
   const PagedTiles list = paged_tiles<MORE>(x, ctx + pf_div(row0, by_G, sG) + 1, kmax,
                                             n_tiles, PF_KT);
   const int tpp = (max(list.n, 0) + parts - 1) / parts;
@@ -428,12 +437,18 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
   // make every wait for LDS a wait for it too. The first are asked for here: what comes
   // before the tile is 0.8 us.
   const int* btab = block_tables + (long)seq * max_blocks;
-  const int last_blk = (seq_len - 1) / PF_BS;
+  const int last_blk = (CACHE8 ? min(seq_len, room) - 1 : seq_len - 1) / PF_BS;
   const int last_row = (seq_len - 1) % PF_BS;
   int tb = 0;                                    // from this one on
+  float2 sizes = {0.0f, 0.0f};                   // of the pages
   auto pages_from = [&](int n) {
-    return btab[min(list.at(i_begin + (n + lane) * KG) * (PF_KT / PF_BS) + wid,
-                    last_blk)];
+    int id = btab[min(list.at(i_begin + (n + lane) * KG) * (PF_KT / PF_BS) + wid,
+                      last_blk)];
+    if constexpr (CACHE8) {                      // an id of no page is page 0
+      id = (unsigned)id < (unsigned)c8.blocks ? id : 0;
+      sizes = c8.scale[(long)id * n_kv + kvh];
+    }
+    return id;
   };
   int pages = 0;
   if (i_begin < i_end) pages = pages_from(0);
@@ -445,8 +460,11 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
   const bool row_ok = rho < rows;
   const int qi = pf_div(rho, by_G, sG);
   const int head = kvh * G + rho - qi * G;
-  const int limit = row_ok ? ctx + qi + 1 : 0;   // keys this row sees
-  const int wmin = ctx + pf_div(wrow0, by_G, sG) + 1;   // fewest of a row in the wave
+  const int limit =                              // keys this row sees
+      row_ok ? (CACHE8 ? min(ctx + qi + 1, room) : ctx + qi + 1) : 0;
+  // fewest of a row in the wave
+  const int wmin = CACHE8 ? min(ctx + pf_div(wrow0, by_G, sG) + 1, room)
+                          : ctx + pf_div(wrow0, by_G, sG) + 1;
   const int wmax = ctx + pf_div(min(wrow0 + 32, rows) - 1, by_G, sG) + 1;
 
   // keys below lo are out of sight but for the kept ones
@@ -507,17 +525,88 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
     }
   };
 
+  // 8 bits: a page of keys and one of values to registers, 16 B a lane, ...
+  constexpr int N8 = CACHE8 ? D / 64 : 1;
+  uint4 k8[N8], v8[N8];
+  float k8s = 0.0f, v8s = 0.0f;
+  auto fetch = [&](int n) {                      // the n-th tile's
+    const int at = n - tb;
+    const long page =
+        (long)__builtin_amdgcn_readlane(pages, at) * n_kv + kvh;
+    k8s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sizes.x), at));
+    v8s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sizes.y), at));
+    const long from = page * (PF_BS * D) + lane * 16;
+#pragma unroll
+    for (int i = 0; i < N8; i++) {
+      k8[i] = *reinterpret_cast<const uint4*>(
+          reinterpret_cast<const char*>(k_cache) + from + i * 1024);
+      v8[i] = *reinterpret_cast<const uint4*>(
+          reinterpret_cast<const char*>(v_cache) + from + i * 1024);
+    }
+  };
+  // ... and from there to their tile
+  auto settle = [&](int t, int buf) {
+    unsigned short* dst = kv_lds + (kg * 2 + buf) * 2 * TILE;
+    const int keys = min(seq_len, room) - (t * (PF_KT / PF_BS) + wid) * PF_BS;
+    // uniform: some row of the workgroup does not see all of the tile
+    const bool edge = t * PF_KT + PF_KT > ctx + pf_div(row0, by_G, sG) + 1;
+    unsigned nan = 0;
+#pragma unroll
+    for (int i = 0; i < N8; i++) {
+      const int p = lane + 64 * i;
+      // keys: chunk p / 16 of 16 channels of token p % 16
+      const int row = wid * PF_BS + (p & 15), c = 2 * (p >> 4);
+      unsigned short* kr = dst + row * D;
+      const int xk = mr_swz_rows<D>(row);
+      *reinterpret_cast<bf16x8*>(kr + ((c ^ xk) << 3)) =
+          kv8_wide(k8[i].x, k8[i].y, k8s);
+      *reinterpret_cast<bf16x8*>(kr + (((c + 1) ^ xk) << 3)) =
+          kv8_wide(k8[i].z, k8[i].w, k8s);
+      // values: 16 tokens of channel p; zeros behind the last key
+      const uint4 v = keys < PF_BS ? kv8_first(v8[i], keys) : v8[i];
+      if (edge) nan |= kv8_nan(v.x) | kv8_nan(v.y) | kv8_nan(v.z) | kv8_nan(v.w);
+      unsigned short* vr = dst + TILE + p * PF_KT;
+      const int xv = mr_swz_rows<PF_KT>(p);
+      *reinterpret_cast<bf16x8*>(vr + (((2 * wid) ^ xv) << 3)) =
+          kv8_wide(v.x, v.y, v8s);
+      *reinterpret_cast<bf16x8*>(vr + (((2 * wid + 1) ^ xv) << 3)) =
+          kv8_wide(v.z, v.w, v8s);
+    }
+    if (edge) {
+      const bool any = __any(nan != 0);
+      if (lane == 0) nan_lds[(kg * 2 + buf) * 4 + wid] = any;
+    }
+  };
+
   const int kbase = mr_row_base<D>(lane), vbase = mr_col_base<D>(lane);
+  const int vbase8 = c32 * PF_KT + ((h ^ mr_swz_rows<PF_KT>(c32)) << 3);
 
   if (i_begin < i_end) {
-    stage(list.at(i_begin), __builtin_amdgcn_readlane(pages, 0), 0);
+    if constexpr (CACHE8) {
+      fetch(0);
+      settle(list.at(i_begin), 0);
+      if (i_begin + KG < i_end) fetch(1);
+    } else {
+      stage(list.at(i_begin), __builtin_amdgcn_readlane(pages, 0), 0);
+    }
   }
   // a step: a tile of every group, the last of which may have none left
   for (int at = p_begin, n = 0; at < i_end; at += KG, n++) {
     const int buf = n & 1, it = at + kg;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (!CACHE8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (it + KG < i_end) {
+    if constexpr (CACHE8) {
+      if (it + KG < i_end) {
+        settle(list.at(it + KG), buf ^ 1);
+        if (it + 2 * KG < i_end) {
+          if (n + 2 - tb == 64) {
+            tb += 64;
+            pages = pages_from(tb);
+          }
+          fetch(n + 2);
+        }
+      }
+    } else if (it + KG < i_end) {
       if (n + 1 - tb == 64) {
         tb += 64;
         pages = pages_from(tb);
@@ -599,11 +688,47 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
         }
       }
     // ---- O^T += V^T P^T ------------------------------------------------------
+    if constexpr (CACHE8) {
+      // A value that is a NaN counts for the rows that see it: 0 times it is one too.
+      const int* nan = nan_lds + (kg * 2 + buf) * 4;
+      if (k0 + PF_KT > wmin && (nan[0] | nan[1] | nan[2] | nan[3]) != 0) {
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) {
+          f32x16 count = mr_zero();              // of those, by row
+#pragma unroll
+          for (int st = 0; st < 4; st++) {
+            bf16x8 a = *reinterpret_cast<const lds_bf16x8*>(
+                vt + (vbase8 ^ (st << 4)) + dt * 32 * PF_KT);
+            bf16x8 is, sees;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              const bool none = (a[j] & 0x7fff) > 0x7f80;
+              is[j] = none ? 0x3f80 : 0;
+              a[j] = none ? (short)0 : a[j];
+              sees[j] = k0 + 16 * st + 8 * h + j < limit ? 0x3f80 : 0;
+            }
+            count = mr_mma(is, sees, count);
+#pragma unroll
+            for (int e = 0; e < TERMS; e++)
+              o_acc[dt] = mr_mma(a, p[e][st], o_acc[dt]);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; r++)
+            if (count[r] > 0.0f) o_acc[dt][r] = NAN;
+        }
+        continue;
+      }
+    }
 #pragma unroll
     for (int st = 0; st < 4; st++)
 #pragma unroll
       for (int dt = 0; dt < DT; dt++) {
-        const bf16x8 a = mr_cols_own<D>(vt + (vbase ^ (dt << 5)) + st * 16 * D);
+        bf16x8 a;
+        if constexpr (CACHE8)
+          a = *reinterpret_cast<const lds_bf16x8*>(vt + (vbase8 ^ (st << 4)) +
+                                                   dt * 32 * PF_KT);
+        else
+          a = mr_cols_own<D>(vt + (vbase ^ (dt << 5)) + st * 16 * D);
 #pragma unroll
         for (int e = 0; e < TERMS; e++)
           o_acc[dt] = mr_mma(a, p[e][st], o_acc[dt]);
@@ -921,15 +1046,16 @@ inline long paged_rows_wgs(const PagedRows& p, long tokens, int n_seqs, int G,
 }
 
 // Prompt rows and the merge of their parts
-template <int D, int TERMS, bool MORE>
-inline void paged_rows(void* out, float* ws_o, const unsigned short* q,
-                       const unsigned short* k_cache,
-                       const unsigned short* v_cache, const int* block_tables,
-                       const int* cu_q, const int* seq_lens, long tokens,
-                       int n_seqs, float scale, int n_qheads, int n_kv,
-                       int max_blocks, long q_stride, long out_stride,
-                       const PagedRows& plan, const PagedMore& x,
-                       const PagedAhead& ahead, hipStream_t stream) {
+template <int D, int TERMS, bool MORE, bool CACHE8>
+inline void paged_rows_of(void* out, float* ws_o, const unsigned short* q,
+                          const unsigned short* k_cache,
+                          const unsigned short* v_cache, const int* block_tables,
+                          const int* cu_q, const int* seq_lens, long tokens,
+                          int n_seqs, float scale, int n_qheads, int n_kv,
+                          int max_blocks, long q_stride, long out_stride,
+                          const PagedRows& plan, const PagedMore& x,
+                          const PagedAhead& ahead, const Kv8Pages& c8,
+                          hipStream_t stream) {
   const int G = n_qheads / n_kv;
   if (tokens == 0 || n_seqs <= 0) return;
   const long wgs = paged_rows_wgs(plan, tokens, n_seqs, G, n_kv);
@@ -943,13 +1069,14 @@ inline void paged_rows(void* out, float* ws_o, const unsigned short* q,
   // 28/4 9.62 -> 9.46 us, 325 drawn ones 0.941 -> 0.934 of the time before there was one.
   const bool as_is = n_seqs > 1 && wgs <= 256;
 #define PF_GO(KG, SPLIT, SORT)                                                 \
-  hipLaunchKernelGGL((paged_attn_rows_kernel<D, TERMS, MORE, KG, SPLIT, SORT>),\
+  hipLaunchKernelGGL((paged_attn_rows_kernel<D, TERMS, MORE, KG, SPLIT, SORT,  \
+                                             CACHE8>),                         \
                      dim3((unsigned)(wgs + ahead.wgs)), dim3(KG * 256), 0,     \
                      stream, block_tables, cu_q, seq_lens, n_seqs, G, n_kv,    \
                      max_blocks, pf_inverse(n_kv), pf_inverse(G), k_cache, q,  \
                      v_cache, out, ws_o, ws_ml, ws_at,                         \
                      meet, scale, q_stride, out_stride, plan.least, plan.most, \
-                     turn, x, ahead)
+                     turn, x, ahead, c8)
   if (plan.groups == 2 && plan.least > 0) PF_GO(2, true, true);
   else if (plan.groups == 2) PF_GO(2, false, true);
   else if (plan.least > 0) PF_GO(1, true, true);
@@ -960,6 +1087,20 @@ inline void paged_rows(void* out, float* ws_o, const unsigned short* q,
     paged_merge<D, MORE, PF_ROWS, PF_KT>(out, ws_o, ws_ml, ws_at, n_qheads, out_stride,
                                          tokens * n_qheads, x, stream, cu_q, seq_lens,
                                          n_seqs, n_kv, plan.most);
+}
+template <int D, int TERMS, bool MORE>
+inline void paged_rows(void* out, float* ws_o, const unsigned short* q,
+                       const unsigned short* k_cache,
+                       const unsigned short* v_cache, const int* block_tables,
+                       const int* cu_q, const int* seq_lens, long tokens,
+                       int n_seqs, float scale, int n_qheads, int n_kv,
+                       int max_blocks, long q_stride, long out_stride,
+                       const PagedRows& plan, const PagedMore& x,
+                       const PagedAhead& ahead, hipStream_t stream) {
+  paged_rows_of<D, TERMS, MORE, false>(
+      out, ws_o, q, k_cache, v_cache, block_tables, cu_q, seq_lens, tokens, n_seqs,
+      scale, n_qheads, n_kv, max_blocks, q_stride, out_stride, plan, x, ahead,
+      Kv8Pages{}, stream);
 }
 
 }  // namespace xllm

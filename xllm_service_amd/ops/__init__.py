@@ -188,6 +188,100 @@ def paged_attn_prefill(q, k_cache, v_cache, block_tables, cu_q, seq_lens,
     return res
 
 
+# ---- paged cache held in 8 bits ----------------------------------------------
+# Keys and values in e4m3, with one power of two as the scale of each page of 16
+# tokens and head (layout and reasons: csrc/ops/kv8.h): half the bytes of a bf16
+# cache, so twice the tokens in the same memory, and decoded rows in half the time.
+def kv8_cache(num_blocks, n_kv, head_dim, device=None):
+    """An empty cache: k_cache [blocks, n_kv, head_dim/16, 16, 16] (chunk of 16
+    channels, token, channel) and v_cache [blocks, n_kv, head_dim, 16] (channel,
+    token) in float8_e4m3fn, kv_scale [blocks, n_kv, 2] in float32 (of the page's
+    keys, of its values). What a page holds is its bytes times its scale; a copy
+    of a page is a copy of its rows in all three. head_dim 64 or 128."""
+    if head_dim not in (64, 128):
+        raise RuntimeError(f"kv8: head_dim 64 or 128, not {head_dim}")
+    f8 = dict(dtype=torch.float8_e4m3fn, device=device)
+    return (torch.zeros(num_blocks, n_kv, head_dim // 16, 16, 16, **f8),
+            torch.zeros(num_blocks, n_kv, head_dim, 16, **f8),
+            torch.zeros(num_blocks, n_kv, 2, device=device))
+
+
+def extend_block_tables(block_tables, seq_lens, new_lens, free_blocks,
+                        num_tokens):
+    """Plan of a step in which sequence i grows from seq_lens[i] to new_lens[i]
+    tokens (int32; a shorter new length counts as the old one), without the host.
+    New pages are taken from free_blocks (int32) in the order of (sequence, page)
+    and written into block_tables (int32 [sequences, columns]) behind the
+    ceil(seq_lens / 16) that each has. Returns, for the new tokens in the order of
+    (sequence, position), slot_mapping and positions (int64 [num_tokens]), cu_q
+    (int32 [sequences + 1]) and the pages taken (int32 [1]).
+
+    num_tokens: room for new tokens, at least their sum. Rows behind the last one
+    have slot -1 and position 0. Pages that free_blocks or a table's columns have no
+    place for are not written and their tokens have slot -1: the step fits if the
+    pages taken are no more than free_blocks has and lengths no more than tables."""
+    if block_tables.is_cuda:
+        _require_ext()
+        return _ops.extend_block_tables(block_tables, seq_lens, new_lens,
+                                        free_blocks, num_tokens)
+    return ref.extend_block_tables(block_tables, seq_lens, new_lens,
+                                   free_blocks, num_tokens)
+
+
+def reshape_and_cache_kv8(k, v, k_cache, v_cache, kv_scale, slot_mapping):
+    """New keys and values [tokens, n_kv, head_dim] into their slots (page * 16 +
+    offset; -1, or outside of the cache: skipped). Tokens of one page must stand
+    side by side in slot_mapping, as those of a sequence do, with none but skipped
+    ones among them; of two for the same slot the later one stays.
+
+    Where the token at offset 0 of a page is among them the page begins anew: its
+    scale is the least power of two whose multiple of 448 holds all of them, and
+    offsets that none of them has become zero. Else its earlier tokens stay, and
+    if the scale has to grow they are rounded to it once more (which changes only
+    those that become subnormal). What is not finite is held as a NaN and does not
+    count for the scale."""
+    if k.is_cuda:
+        _require_ext()
+        _ops.reshape_and_cache_kv8(k, v, k_cache, v_cache, kv_scale,
+                                   slot_mapping)
+        return
+    ref.reshape_and_cache_kv8(k, v, k_cache, v_cache, kv_scale, slot_mapping)
+
+
+def paged_attn_decode_kv8(q, k_cache, v_cache, kv_scale, block_tables, seq_lens,
+                          scale, out=None):
+    """`paged_attn_decode` over a cache held in 8 bits: q [sequences, heads,
+    head_dim] bf16, at most 16 heads for each of the cache's. Sequences without
+    keys give zeros. Entries of a table that name no page count as page 0, tokens
+    behind the end of a table do not count."""
+    if q.is_cuda:
+        _require_ext()
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _ops.paged_attn_decode_kv8(out, q, k_cache, v_cache, kv_scale,
+                                   block_tables, seq_lens, scale)
+        return out
+    return ref.paged_attn_decode_kv8(q, k_cache, v_cache, kv_scale, block_tables,
+                                     seq_lens, scale, out)
+
+
+def paged_attn_prefill_kv8(q, k_cache, v_cache, kv_scale, block_tables, cu_q,
+                           seq_lens, scale, out=None):
+    """`paged_attn_prefill` over a cache held in 8 bits: q [tokens, heads,
+    head_dim] bf16, those of sequence i from cu_q[i] to cu_q[i + 1]; causal, the
+    last of them sees all seq_lens[i] keys. Rows that see no key give zeros, rows
+    behind the last sequence stay as they were. Tables as for decoded rows."""
+    if q.is_cuda:
+        _require_ext()
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _ops.paged_attn_prefill_kv8(out, q, k_cache, v_cache, kv_scale,
+                                    block_tables, cu_q, seq_lens, scale)
+        return out
+    return ref.paged_attn_prefill_kv8(q, k_cache, v_cache, kv_scale,
+                                      block_tables, cu_q, seq_lens, scale, out)
+
+
 def greedy_sample(logits: torch.Tensor) -> torch.Tensor:
     if logits.is_cuda:
         _require_ext()

@@ -160,6 +160,167 @@ def paged_attn_prefill(q, k_cache, v_cache, block_tables, cu_q, seq_lens, scale)
     return out
 
 
+# ---- paged cache held in 8 bits (csrc/ops/kv8.h) -----------------------------
+KV8_PAGE = 16
+
+
+def extend_block_tables(block_tables, seq_lens, new_lens, free_blocks,
+                        num_tokens):
+    W, F = block_tables.shape[1], free_blocks.shape[0]
+    slots = torch.full((num_tokens,), -1, dtype=torch.long)
+    positions = torch.zeros(num_tokens, dtype=torch.long)
+    cu_q = [0]
+    at = pages = 0
+    for i, (old, new) in enumerate(zip(seq_lens.tolist(), new_lens.tolist())):
+        old = max(old, 0)
+        new = max(new, old)
+        held, need = -(-old // KV8_PAGE), -(-new // KV8_PAGE)
+        for col in range(held, min(need, W)):
+            if pages + col - held < F:
+                block_tables[i, col] = free_blocks[pages + col - held]
+        for pos in range(old, min(new, old + num_tokens - at)):
+            col = pos // KV8_PAGE
+            known = col < W and (col < held or pages + col - held < F)
+            page = int(block_tables[i, col]) if known else -1
+            if page >= 0:
+                slots[at + pos - old] = page * KV8_PAGE + pos % KV8_PAGE
+            positions[at + pos - old] = pos
+        at = min(at + new - old, num_tokens)
+        pages += need - held
+        cu_q.append(at)
+    return (slots, positions, torch.tensor(cu_q, dtype=torch.int32),
+            torch.tensor([pages], dtype=torch.int32))
+
+
+def kv8_shape(k_cache, v_cache, kv_scale):
+    """(pages, heads, head_dim) of a cache; its argument checks."""
+    f8 = torch.float8_e4m3fn
+    if not (k_cache.dtype == v_cache.dtype == f8
+            and kv_scale.dtype == torch.float32):
+        raise RuntimeError("kv8: caches must be float8_e4m3fn, kv_scale float32")
+    if not all(t.is_contiguous() for t in (k_cache, v_cache, kv_scale)):
+        raise RuntimeError("kv8: the cache must be contiguous")
+    if v_cache.dim() != 4 or v_cache.shape[2] not in (64, 128):
+        raise RuntimeError("kv8: head_dim 64 or 128")
+    B, KV, D, _ = v_cache.shape
+    if not (B and KV and v_cache.shape[3] == KV8_PAGE
+            and k_cache.shape == (B, KV, D // 16, KV8_PAGE, 16)
+            and kv_scale.shape == (B, KV, 2)):
+        raise RuntimeError("kv8: shapes of the cache do not match")
+    return B, KV, D
+
+
+def kv8_values(k_cache, v_cache, kv_scale):
+    """Keys and values that a cache holds, fp32 [pages, heads, 16, head_dim]."""
+    B, KV, D = kv8_shape(k_cache, v_cache, kv_scale)
+    k = k_cache.float().transpose(2, 3).reshape(B, KV, KV8_PAGE, D)
+    v = v_cache.float().transpose(2, 3)
+    return (k * kv_scale[..., 0, None, None], v * kv_scale[..., 1, None, None])
+
+
+def _kv8_fit(x):
+    """The least power of two from 2^-126 on whose multiple of 448 holds the
+    finite values of x [tokens, heads, D]; fp32 [heads]."""
+    big = torch.where(x.isfinite(), x, torch.zeros_like(x)).abs().amax((0, 2))
+    m, e = torch.frexp(big)
+    e = torch.where(m > 0, e - 9 + (m > 0.875), -126)
+    return torch.exp2(e.clamp(min=-126).float())
+
+
+def reshape_and_cache_kv8(k, v, k_cache, v_cache, kv_scale, slot_mapping):
+    B, KV, D = kv8_shape(k_cache, v_cache, kv_scale)
+    T = slot_mapping.shape[0]
+    if k.shape != (T, KV, D) or v.shape != (T, KV, D):
+        raise RuntimeError("kv8: k and v must have the cache's heads, and a "
+                           "row for each token")
+    if slot_mapping.dtype != torch.long or slot_mapping.dim() != 1:
+        raise RuntimeError("kv8: slot_mapping must be int64")
+    on = (slot_mapping >= 0) & (slot_mapping < B * KV8_PAGE)
+    k, v, slots = k[on], v[on], slot_mapping[on].tolist()
+    f8, t0, T = torch.float8_e4m3fn, 0, len(slots)
+    # (float8 tensors are written through their bytes)
+    raw = (k_cache.view(torch.uint8), v_cache.view(torch.uint8))
+    while t0 < T:
+        page = slots[t0] // KV8_PAGE
+        t1 = t0 + 1
+        while t1 < T and slots[t1] // KV8_PAGE == page:
+            t1 += 1
+        offs = [s % KV8_PAGE for s in slots[t0:t1]]
+        for i, x in enumerate((k, v)):
+            x = x[t0:t1].float()
+            now = _kv8_fit(x)
+            if 0 in offs:
+                raw[i][page] = 0
+            else:
+                was = kv_scale[page, :, i]
+                now = torch.maximum(was, now)
+                kept = raw[i][page].view(f8).float()
+                by = (was / now).reshape(KV, *[1] * (kept.dim() - 1))
+                raw[i][page] = (kept * by).to(f8).view(torch.uint8)
+            kv_scale[page, :, i] = now
+            x = torch.where(x.isfinite(), x / now[None, :, None],
+                            torch.full_like(x, float("nan"))).to(f8)
+            x = x.view(torch.uint8)
+            for j, o in enumerate(offs):
+                if i == 0:
+                    raw[i][page, :, :, o] = x[j].unflatten(1, (D // 16, 16))
+                else:
+                    raw[i][page, :, :, o] = x[j]
+        t0 = t1
+
+
+def _kv8_check_attention(q, cache, block_tables, lens, n_seqs):
+    B, KV, D = kv8_shape(*cache)
+    if q.dim() != 3 or q.shape[2] != D or not q.shape[1] or q.shape[1] % KV:
+        raise RuntimeError("kv8: q must be [tokens, heads, head_dim] with a "
+                           "multiple of the cache's heads")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 \
+            or lens.dtype != torch.int32 or lens.dim() != 1 \
+            or block_tables.shape[0] < n_seqs or lens.shape[0] < n_seqs:
+        raise RuntimeError("kv8: an int32 table and length for each sequence")
+
+
+def paged_attn_prefill_kv8(q, k_cache, v_cache, kv_scale, block_tables, cu_q,
+                           seq_lens, scale, out=None):
+    cache = (k_cache, v_cache, kv_scale)
+    if cu_q.dtype != torch.int32 or cu_q.dim() != 1 or cu_q.shape[0] < 1:
+        raise RuntimeError("kv8: cu_q must be int32")
+    _kv8_check_attention(q, cache, block_tables, seq_lens, cu_q.shape[0] - 1)
+    k, v = kv8_values(*cache)
+    B, KV, _, D = k.shape
+    G = q.shape[1] // KV
+    out = torch.zeros_like(q) if out is None else out
+    cu = cu_q.tolist()
+    for s, (q0, q1) in enumerate(zip(cu[:-1], cu[1:])):
+        total = int(seq_lens[s])
+        L = max(min(total, block_tables.shape[1] * KV8_PAGE), 0)
+        ids = block_tables[s, :-(-L // KV8_PAGE)].long()
+        ids = torch.where((ids >= 0) & (ids < B), ids, 0)
+        seen = torch.arange(L) <= (total - (q1 - q0)
+                                   + torch.arange(q1 - q0))[:, None]
+        for h in range(q.shape[1]):
+            kk = k[ids, h // G].reshape(-1, D)[:L]
+            vv = v[ids, h // G].reshape(-1, D)[:L]
+            z = (q[q0:q1, h].float() @ kk.T) * scale
+            p = torch.softmax(z.masked_fill(~seen, float("-inf")), -1)
+            p = torch.where(seen.any(-1, keepdim=True), p, 0.0)
+            out[q0:q1, h] = (p @ vv).to(q.dtype)
+    return out
+
+
+def paged_attn_decode_kv8(q, k_cache, v_cache, kv_scale, block_tables, seq_lens,
+                          scale, out=None):
+    S = q.shape[0]
+    _, KV, _ = kv8_shape(k_cache, v_cache, kv_scale)
+    if q.dim() == 3 and q.shape[1] > 16 * KV:
+        raise RuntimeError("kv8: at most 16 query heads for each of the cache's")
+    _kv8_check_attention(q, (k_cache, v_cache, kv_scale), block_tables, seq_lens,
+                         S)
+    return paged_attn_prefill_kv8(
+        q, k_cache, v_cache, kv_scale, block_tables[:S],
+        torch.arange(S + 1, dtype=torch.int32), seq_lens[:S], scale, out)
+
+
 def greedy_sample(logits: torch.Tensor) -> torch.Tensor:
     return logits.float().argmax(dim=-1)
 
