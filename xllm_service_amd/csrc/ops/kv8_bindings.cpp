@@ -12,7 +12,7 @@ void launch_kv8_plan(int*, const int*, const int*, const int*, long*, long*, int
                      int*, int, int, long, int, int, hipStream_t);
 void launch_kv8_write(unsigned char*, unsigned char*, float*, const unsigned short*,
                       const unsigned short*, const long*, int, int, int, long, long,
-                      long, hipStream_t);
+                      int, hipStream_t);
 int kv8_decode_parts(int, int, int);
 void launch_kv8_decode(unsigned short*, const unsigned short*, const unsigned char*,
                        const unsigned char*, const float*, const int*, const int*,
@@ -103,11 +103,12 @@ void write_pages(Tensor k, Tensor v, Tensor k_cache, Tensor v_cache, Tensor kv_s
                   slots.size(0) == k.size(0),
               "kv8: slot_mapping must be contiguous int64, one for each token");
   if (k.size(0) == 0) return;
-  // keys are read by 16 B: a copy of what lies at other addresses
+  // keys are read by 16 B, values by 4: copies of what lies at other addresses
   if (!on_bytes(k, 16)) k = k.clone(at::MemoryFormat::Contiguous);
+  if (!on_bytes(v, 4)) v = v.clone(at::MemoryFormat::Contiguous);
   xllm::launch_kv8_write(bytes(k_cache), bytes(v_cache), kv_scale.data_ptr<float>(),
                          words(k), words(v), slots.data_ptr<long>(), (int)k.size(0),
-                         c.n_kv, c.D, k.stride(0), v.stride(0), c.blocks * 16L,
+                         c.n_kv, c.D, k.stride(0), v.stride(0), c.blocks,
                          stream_of(kv_scale));
 }
 
@@ -213,11 +214,21 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> plan_tables(Tensor tables, Tensor seq
   TORCH_CHECK(n_tokens >= 0 && n_tokens < (1L << 30) && S < (1L << 24) &&
                   tables.size(1) < (1L << 26) && free_blocks.size(0) < (1L << 30),
               "too many tokens, sequences or pages");
-  const auto longs = tables.options().dtype(torch::kLong);
-  auto slots = torch::empty({n_tokens}, longs);
-  auto positions = torch::empty({n_tokens}, longs);
-  auto cu_q = torch::empty({S + 1}, tables.options());
-  auto used = torch::empty({1}, tables.options());
+  // one piece of memory for all four: an allocation takes 1.2 us
+  const auto all = torch::empty({2 * n_tokens + (S + 3) / 2},
+                                tables.options().dtype(torch::kLong));
+  auto piece = [&](caffe2::TypeMeta type, long from, long n) {
+    auto t = at::detail::make_tensor<c10::TensorImpl>(
+        c10::Storage(all.storage()), all.key_set(), type);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    t.unsafeGetTensorImpl()->set_storage_offset(from);
+    return t;
+  };
+  const auto longs = all.dtype(), ints = tables.dtype();
+  auto slots = piece(longs, 0, n_tokens);
+  auto positions = piece(longs, n_tokens, n_tokens);
+  auto cu_q = piece(ints, 4 * n_tokens, S + 1);
+  auto used = piece(ints, 4 * n_tokens + S + 1, 1);
   xllm::launch_kv8_plan(
       tables.data_ptr<int>(), seq_lens.data_ptr<int>(), new_lens.data_ptr<int>(),
       free_blocks.data_ptr<int>(), slots.data_ptr<long>(),

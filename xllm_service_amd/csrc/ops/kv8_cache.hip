@@ -2,7 +2,7 @@
 // step's new tokens, and their keys and values.
 #include <algorithm>
 
-#include "kv8.h"
+#include "paged_rows.h"
 
 namespace xllm {
 
@@ -11,34 +11,33 @@ namespace xllm {
 // the order of (sequence, page), its new tokens stand in the order of (sequence,
 // position); both offsets are sums over the sequences before it. Integers only, a few
 // KB: bound by a launch and the chain lengths -> sums -> ids -> stores. So every
-// workgroup makes the sums for itself, 256 sequences at a time, instead of waiting for
+// workgroup makes the sums for itself, a sequence to a thread, instead of waiting for
 // another one's, and writes its share of tokens and pages, which it finds by halves.
-constexpr int KV8_SEQS = 256;              // sequences of a round, threads
-
-__global__ __launch_bounds__(KV8_SEQS) void kv8_plan_kernel(
+// Us in a captured graph, where a launch takes 3.2: one sequence 3.3, 128 that grow by a
+// token 4.1, 600 by 36 k tokens 5.8, 1000 by 39 k 6.0. A call from the host takes 5.5,
+// with the memory of its results.
+// SEQS: sequences of a round, threads.
+template <int SEQS>
+__global__ __launch_bounds__(SEQS) void kv8_plan_kernel(
     int* __restrict__ tables, const int* __restrict__ seq_lens,
     const int* __restrict__ new_lens, const int* __restrict__ free_blocks,
     long* __restrict__ slots, long* __restrict__ positions,
     int* __restrict__ cu_q, int* __restrict__ used, const int n_seqs,
     const int width, const long table_stride, const int n_free,
     const int n_tokens) {
-  __shared__ int tok_at[KV8_SEQS + 1], page_at[KV8_SEQS + 1], had[KV8_SEQS];
-  __shared__ int sums[2][KV8_SEQS / 64];
+  __shared__ int tok_at[SEQS + 1], page_at[SEQS + 1], had[SEQS];
+  __shared__ int sums[2][SEQS / 64];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int groups = gridDim.x, me = blockIdx.x;
   int tokens = 0, pages = 0;               // of the rounds before
-  for (int base = 0; base < n_seqs; base += KV8_SEQS) {
+  for (int base = 0; base < n_seqs; base += SEQS) {
     const int i = base + tid;
     const int old = i < n_seqs ? max(seq_lens[i], 0) : 0;
     const int now = i < n_seqs ? max(new_lens[i], old) : 0;
     const int first = old / KV8_PAGE + (old % KV8_PAGE != 0);
-    int t = now - old, p = now / KV8_PAGE + (now % KV8_PAGE != 0) - first;
-    const int mine_t = t, mine_p = p;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int ut = __shfl_up(t, off, 64), up = __shfl_up(p, off, 64);
-      if (lane >= off) t += ut, p += up;
-    }
+    const int mine_t = now - old;
+    int t = pf_scan<true>(mine_t);
+    int p = pf_scan<true>(now / KV8_PAGE + (now % KV8_PAGE != 0) - first);
     if (lane == 63) sums[0][wid] = t, sums[1][wid] = p;
     __syncthreads();
     for (int w = 0; w < wid; w++) t += sums[0][w], p += sums[1][w];
@@ -48,22 +47,22 @@ __global__ __launch_bounds__(KV8_SEQS) void kv8_plan_kernel(
     if (tid == 0) tok_at[0] = tokens, page_at[0] = pages;
     if (me == 0 && i < n_seqs) cu_q[i] = min(tokens + t - mine_t, n_tokens);
     __syncthreads();
-    const int n = min(n_seqs - base, KV8_SEQS);
+    const int n = min(n_seqs - base, SEQS);
     // the sequence of this round that entry x of a list of sums is in
     auto find = [&](const int* at, int x) {
       int lo = 0;
 #pragma unroll
-      for (int step = KV8_SEQS / 2; step > 0; step >>= 1)
+      for (int step = SEQS / 2; step > 0; step >>= 1)
         if (lo + step < n && at[lo + step] <= x) lo += step;
       return lo;
     };
     // chunks of 256, every groups-th of them
     auto mine = [&](int from) {
-      const int c = from / KV8_SEQS, ahead = (me - c % groups + groups) % groups;
-      return (c + ahead) * KV8_SEQS + tid;
+      const int c = from / SEQS, ahead = (me - c % groups + groups) % groups;
+      return (c + ahead) * SEQS + tid;
     };
     const int t1 = min(tok_at[n], n_tokens);
-    for (int x = mine(tok_at[0]); x < t1; x += groups * KV8_SEQS) {
+    for (int x = mine(tok_at[0]); x < t1; x += groups * SEQS) {
       if (x < tok_at[0]) continue;
       const int s = find(tok_at, x), pos = had[s] + x - tok_at[s];
       const int col = pos / KV8_PAGE;
@@ -78,15 +77,15 @@ __global__ __launch_bounds__(KV8_SEQS) void kv8_plan_kernel(
       positions[x] = pos;
     }
     const int p1 = min(page_at[n], n_free);
-    for (int x = mine(page_at[0]); x < p1; x += groups * KV8_SEQS) {
+    for (int x = mine(page_at[0]); x < p1; x += groups * SEQS) {
       if (x < page_at[0]) continue;
       const int s = find(page_at, x);
       const int col = had[s] / KV8_PAGE + (had[s] % KV8_PAGE != 0) + x - page_at[s];
       if ((unsigned)col < (unsigned)width)
         tables[(base + s) * table_stride + col] = free_blocks[x];
     }
-    tokens = tok_at[KV8_SEQS];
-    pages = page_at[KV8_SEQS];
+    tokens = tok_at[SEQS];
+    pages = page_at[SEQS];
     __syncthreads();
   }
   if (me == 0 && tid == 0) {
@@ -94,7 +93,7 @@ __global__ __launch_bounds__(KV8_SEQS) void kv8_plan_kernel(
     *used = pages;
   }
   // rows behind the last token
-  for (int x = tokens + me * KV8_SEQS + tid; x < n_tokens; x += groups * KV8_SEQS) {
+  for (int x = tokens + me * SEQS + tid; x < n_tokens; x += groups * SEQS) {
     slots[x] = -1;
     positions[x] = 0;
   }
@@ -106,153 +105,286 @@ void launch_kv8_plan(int* tables, const int* seq_lens, const int* new_lens,
                      long table_stride, int n_free, int n_tokens,
                      hipStream_t stream) {
   const long most = std::max<long>(n_tokens, n_seqs);
-  const int groups = (int)std::min<long>(256, most / KV8_SEQS + 1);
-  hipLaunchKernelGGL(kv8_plan_kernel, dim3(groups), dim3(KV8_SEQS), 0, stream,
-                     tables, seq_lens, new_lens, free_blocks, slots, positions,
-                     cu_q, used, n_seqs, width, table_stride, n_free, n_tokens);
+  // more than one round of 256: 300 sequences 5.7 | 4.9 us, 1000 8.5 | 5.1; 128 4.1 | 4.6
+  const int threads = n_seqs <= 256 ? 256 : 1024;
+  const int groups = (int)std::min<long>(256, most / threads + 1);
+  auto go = threads == 256 ? kv8_plan_kernel<256> : kv8_plan_kernel<1024>;
+  hipLaunchKernelGGL(go, dim3(groups), dim3(threads), 0, stream, tables, seq_lens,
+                     new_lens, free_blocks, slots, positions, cu_q, used, n_seqs, width,
+                     table_stride, n_free, n_tokens);
 }
 
 // ---- keys and values ---------------------------------------------------------------
 // A page's new tokens stand side by side in slot_mapping, but for skipped ones among
-// them. The first of them has its page's waves, two for each head, keys and values, which read all of them, make
-// the page's scale and write it: no two waves write to one page, no atomics, one pass.
-// With the page's first token among them the page begins anew, and what none of them
-// writes is zero; else its earlier tokens stay, rounded again if the scale has grown.
-template <int D>
-__global__ __launch_bounds__(256) void kv8_write_kernel(
-    unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache,
-    float* __restrict__ kv_scale, const unsigned short* __restrict__ k,
-    const unsigned short* __restrict__ v, const long* __restrict__ slots,
-    const int n_tokens, const int n_kv, const long k_stride, const long v_stride,
-    const long n_slots) {
+// them: a run. A run has waves of its own, one for each head, keys and values, which
+// read all of it, make the page's scale and write the page: no two waves write to one
+// page, no atomics, one pass. With the page's first token in the run the page begins
+// anew, and what none of its tokens writes is zero; else its earlier tokens stay, rounded
+// again if the scale has grown.
+//
+// A wave looks a window of tokens over and takes the runs that begin there, one after the
+// other, the next one's values on the way meanwhile. Long windows cost tokens that are a
+// run each (1.2 us a run: a wave alone on its SIMD issues its 350 instructions in that),
+// short ones waves that find no run, of which 126 k take 25 us to come and go. Us, windows
+// of 1 | 2 | 4 | 8 | 16, 8 heads of 128: 7878 tokens of four prompts 28 | 21 | 15.7 | 11.9 |
+// 11.5, 2000 of one 25 | 15.7 | 9.9 | 6.6 | 5.5, 300 4.9 | 4.4 | 4.4 | 4.3 | 4.3; a token each
+// of 1000 sequences 14.5 | 15.1 | 14.6 | 17.2 | 25, of 256 5.9 | 6.6 | 8.6 | 13.5 | 23.5, of 128
+// 4.4 | 5.3 | 7.7 | 12.5 | 22. One token: 3.7, a launch.
+//   7878 tokens are 48 MB: 4.1 TB/s, of the 4.97 of a large copy. Before, by a wave to each
+// token and conversions of each value by itself, 47.4.
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+
+template <int D, bool VAL>
+XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
+                             const int n_kv, const int head, const int window,
+                             const unsigned n_blocks,
+                             const unsigned short* __restrict__ rows,
+                             const long stride, float* __restrict__ kv_scale,
+                             unsigned char* __restrict__ cache) {
   constexpr int NP = D / 64;               // 16 B of the page per lane
   const int lane = threadIdx.x & 63;
-  const int t0 = blockIdx.x;
-  const int unit = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 +
-                                                  (threadIdx.x >> 6));
-  const int head = unit >> 1, val = unit & 1;
-  if (head >= n_kv) return;
-  auto page_of = [&](int t) {              // -1: none
+  // page * 16 + offset of a token, -1: skipped
+  auto slot_at = [&](int t) {
+    if (t < 0 || t >= n_tokens) return -1L;
     const long s = slots[t];
-    return s >= 0 && s < n_slots ? s / KV8_PAGE : -1L;
+    return (unsigned long)s < (unsigned long)n_blocks * KV8_PAGE ? s : -1L;
   };
-  const long page = page_of(t0);
-  if (page < 0) return;
-  for (int end = t0; end > 0; end -= 64) {  // the last token before that has a page
-    const int t = end - 64 + lane;
-    const long p = t >= 0 ? page_of(t) : -1L;
-    const unsigned long long any = __ballot(p >= 0);
-    if (any == 0) continue;
-    if (__ballot(p == page) >> (63 - __clzll(any)) & 1) return;
-    break;
-  }
-  const long at = page * n_kv + head;
-  const float was = kv_scale[2 * at + val];
-  // lane o < 16: the last token that is written to offset o, -1: none
-  int src = -1;
-  for (int base = t0; base < n_tokens; base += 64) {
-    const int t = base + lane;
-    const long p = t < n_tokens ? page_of(t) : -1L;
-    // of tokens with another page, the first
-    const unsigned long long out = __ballot(p >= 0 && p != page);
-    const int n = out == 0 ? 64 : __ffsll(out) - 1;
-    const int off = p == page ? (int)(slots[t] % KV8_PAGE) : -1;
-    unsigned long long in = __ballot(p == page && lane < n);
-    for (; in != 0; in &= in - 1) {
-      const int j = __builtin_amdgcn_readfirstlane(__ffsll(in) - 1);
-      if (lane == __builtin_amdgcn_readlane(off, j)) src = base + j;
+  auto page_of = [](long slot) { return slot < 0 ? -1 : (int)(slot / KV8_PAGE); };
+  // lane i has token base + i: the window, one before it, and what follows
+  const int base = (int)blockIdx.x * window - 1;
+  const long slot = slot_at(base + lane);
+  const int page = page_of(slot), off = (int)(slot & (KV8_PAGE - 1));
+  typedef unsigned long long mask;
+  const mask on = __ballot(page >= 0);
+  const mask before = on & ((1ull << lane) - 1);
+  const int last = 63 - __clzll(before | 1);
+  int prev = __shfl(page, last, 64);
+  if (before == 0) prev = -1;
+  mask begins = ((2ull << window) - 2) & on;
+  if (begins == 0) return;
+  if (!(on & 1) && base > 0) {             // only skipped ones: it is further up
+    int found = -1;
+    for (int end = base; end > 0 && found < 0; end -= 64) {
+      const int p = page_of(slot_at(end - 64 + lane));
+      const mask any = __ballot(p >= 0);
+      if (any != 0) found = __builtin_amdgcn_readlane(p, 63 - __clzll(any));
     }
-    if (n < 64) break;
+    if (before == 0) prev = found;
   }
-  const unsigned have = (unsigned)__ballot(src >= 0);
-  const bool anew = have & 1;
-  unsigned char* to = (val ? v_cache : k_cache) + at * (KV8_PAGE * D);
-  // this lane's 16 values of the page, NP times
-  float x[NP][16];
-  uint4 old[NP];
-  int tok[NP];                             // keys: token of the values
-  float big = 0.0f;
-  auto take = [&](float f, float& y) {
-    y = f;
-    const float a = fabsf(f);
-    big = fmaxf(big, a < INFINITY ? a : 0.0f);
+  begins &= __ballot(page != prev);
+  if (begins == 0) return;
+
+  struct Run {                             // on its way
+    unsigned raw[8 * NP];                  // this lane's new values, in bf16: keys, 16
+                                           // channels of a token; values, NP
+                                           // neighbouring channels of 16 tokens
+    uint4 old[NP];                         // 16 B of the page as it was
+    bool fresh[NP];                        // keys: these are new
+    long at;                               // page and head
+    float was;                             // scale
+    unsigned have;                         // offsets with a new token
   };
-#pragma unroll
-  for (int i = 0; i < NP; i++) {
-    const int p = lane + 64 * i;           // 16 B of the page
-    old[i] = make_uint4(0, 0, 0, 0);
-    if (!anew && have != 0xffff)
-      old[i] = *reinterpret_cast<const uint4*>(to + p * 16);
-    if (!val) {                            // chunk p / 16 of token p % 16
-      tok[i] = __shfl(src, p & 15, 64);
-      if (tok[i] >= 0) {
-        const unsigned short* from =
-            k + tok[i] * k_stride + (long)head * D + (p >> 4) * 16;
-        const ushort8_t a = *reinterpret_cast<const ushort8_t*>(from);
-        const ushort8_t b = *reinterpret_cast<const ushort8_t*>(from + 8);
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          take(bf16_to_f32(a.x[j]), x[i][j]);
-          take(bf16_to_f32(b.x[j]), x[i][8 + j]);
+  auto place_of = [&](int i) { return 16 * (VAL ? NP * lane + i : lane + 64 * i); };
+  auto load = [&](Run& r) {                // the next one
+    const int j = __builtin_amdgcn_readfirstlane(__ffsll(begins) - 1);
+    begins &= begins - 1;
+    const int id = __builtin_amdgcn_readlane(page, j);
+    r.at = (long)id * n_kv + head;
+    r.was = kv_scale[2 * r.at + VAL];
+    // its page's tokens up to the next one of another page
+    const mask up = ~0ull << j;
+    const mask other = __ballot(page >= 0 && page != id) & up;
+    const int end = other == 0 ? 64 : __builtin_amdgcn_readfirstlane(__ffsll(other) - 1);
+    const mask in = __ballot(page == id) & up & (end == 64 ? ~0ull : (1ull << end) - 1);
+    int src = -1;                          // lane o < 16: offset o's last token
+    const int off0 = __builtin_amdgcn_readlane(off, j);
+    const int n = __popcll(in);
+    if (end < 64 && in == ((1ull << n) - 1) << j &&
+        (__ballot(off == off0 + lane - j) & in) == in) {
+      // tokens one after the other
+      if (lane >= off0 && lane < off0 + n) src = base + j + lane - off0;
+    } else {
+      auto place = [&](mask m, int o, int from) {
+        for (; m != 0; m &= m - 1) {
+          const int i = __builtin_amdgcn_readfirstlane(__ffsll(m) - 1);
+          if (lane == __builtin_amdgcn_readlane(o, i)) src = from + i;
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; j++) x[i][j] = 0.0f;
+      };
+      place(in, off, base);
+      for (int b = base + 64; end == 64 && b < n_tokens; b += 64) {
+        const long s = slot_at(b + lane);
+        const int p = page_of(s);
+        const mask out = __ballot(p >= 0 && p != id);
+        const mask m = __ballot(p == id);
+        place(out == 0 ? m : m & ((out & -out) - 1), (int)(s & (KV8_PAGE - 1)), b);
+        if (out != 0) break;
       }
-    } else {                               // channel p
+    }
+    r.have = (unsigned)__ballot(src >= 0);
+    const unsigned char* to = cache + r.at * (KV8_PAGE * D);
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+      r.old[i] = make_uint4(0, 0, 0, 0);
+      if (!(r.have & 1)) r.old[i] = *reinterpret_cast<const uint4*>(to + place_of(i));
+    }
+#pragma unroll
+    for (int o = 0; o < 8 * NP; o++) r.raw[o] = 0;
+    if constexpr (!VAL) {
+#pragma unroll
+      for (int i = 0; i < NP; i++) {
+        const int p = lane + 64 * i;       // chunk p / 16 of token p % 16
+        const int t = __shfl(src, p & 15, 64);
+        r.fresh[i] = t >= 0;
+        if (t >= 0) {
+          const uint4* from = reinterpret_cast<const uint4*>(
+              rows + t * stride + (long)head * D + (p >> 4) * 16);
+          const uint4 a = from[0], b = from[1];
+          r.raw[8 * i] = a.x, r.raw[8 * i + 1] = a.y;
+          r.raw[8 * i + 2] = a.z, r.raw[8 * i + 3] = a.w;
+          r.raw[8 * i + 4] = b.x, r.raw[8 * i + 5] = b.y;
+          r.raw[8 * i + 6] = b.z, r.raw[8 * i + 7] = b.w;
+        }
+      }
+    } else {
+      const unsigned short* from = rows + (long)head * D + NP * lane;
 #pragma unroll
       for (int o = 0; o < 16; o++) {
-        x[i][o] = 0.0f;
-        if (have >> o & 1) {               // uniform
-          const int t = __builtin_amdgcn_readlane(src, o);
-          take(bf16_to_f32(v[t * v_stride + (long)head * D + p]), x[i][o]);
+        if (r.have >> o & 1) {             // uniform
+          const long t = __builtin_amdgcn_readlane(src, o);
+          if constexpr (NP == 2)
+            r.raw[o] = *reinterpret_cast<const unsigned*>(from + t * stride);
+          else
+            r.raw[o / 2] |= (unsigned)from[t * stride] << (16 * (o & 1));
         }
       }
     }
-  }
-  const int e = kv8_exponent(wave_reduce_max(big));
-  const float fit = kv8_power(e);
-  const float now = anew ? fit : fmaxf(was, fit);
-  const float by = 1.0f / now;             // exact: a power of two
-  const float again = was / now;           // below 1 where the scale has grown
+  };
+  auto store = [&](const Run& r) {
+    // two values to a word, in the order of the page's bytes
+    unsigned x[NP][8];
 #pragma unroll
-  for (int i = 0; i < NP; i++) {
-    const int p = lane + 64 * i;
-    const bool fresh = val || tok[i] >= 0;
-    unsigned u[4];
-    const unsigned w[4] = {old[i].x, old[i].y, old[i].z, old[i].w};
+    for (int i = 0; i < NP; i++)
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const unsigned kept = again == 1.0f ? w[j] : kv8_again(w[j], again);
-      const unsigned made =
-          fresh ? kv8_pack(x[i][4 * j] * by, x[i][4 * j + 1] * by,
-                           x[i][4 * j + 2] * by, x[i][4 * j + 3] * by)
-                : 0;
-      unsigned mask = fresh ? ~0u : 0;     // bytes that are new
-      if (val) {
-        mask = 0;
+      for (int c = 0; c < 8; c++)
+        x[i][c] = !VAL || NP == 1
+                      ? r.raw[8 * i + c]
+                      : __builtin_amdgcn_perm(r.raw[(2 * c + 1) % (8 * NP)],
+                                              r.raw[(2 * c) % (8 * NP)],
+                                              i ? 0x07060302u : 0x05040100u);
+    // sizes of bf16 sort like their bits
+    u16x2 two = {0, 0};
 #pragma unroll
-        for (int b = 0; b < 4; b++)
-          if (have >> (4 * j + b) & 1) mask |= 255u << (8 * b);
-      }
-      u[j] = (made & mask) | (anew ? 0 : kept & ~mask);
+    for (int i = 0; i < NP; i++)
+#pragma unroll
+      for (int c = 0; c < 8; c++)
+        two = __builtin_elementwise_max(
+            two, __builtin_bit_cast(u16x2, x[i][c] & 0x7fff7fffu));
+    int big = __builtin_amdgcn_readlane(pf_scan<false>(max(two[0], two[1])), 63);
+    const bool odd = big >= 0x7f80;        // uniform: not all finite
+    if (odd) {
+      big = 0;
+#pragma unroll
+      for (int i = 0; i < NP; i++)
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int a = (int)(x[i][c] >> (16 * e)) & 0x7fff;
+            big = max(big, a < 0x7f80 ? a : 0);
+          }
+      big = __builtin_amdgcn_readlane(pf_scan<false>(big), 63);
     }
-    if (fresh || anew || again != 1.0f)
-      *reinterpret_cast<uint4*>(to + p * 16) = make_uint4(u[0], u[1], u[2], u[3]);
+    const bool anew = r.have & 1;
+    const float fit = kv8_power(kv8_exponent(__int_as_float(big << 16)));
+    const float now = anew ? fit : fmaxf(r.was, fit);
+    const float by = 1.0f / now;           // exact: a power of two
+    const float again = r.was / now;       // below 1 where the scale has grown
+    const bool keep = __builtin_amdgcn_readfirstlane(again == 1.0f);
+    unsigned char* to = cache + r.at * (KV8_PAGE * D);
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+      const bool fresh = VAL || r.fresh[i];
+      unsigned u[4], w[4] = {r.old[i].x, r.old[i].y, r.old[i].z, r.old[i].w};
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const unsigned a = x[i][2 * c], b = x[i][2 * c + 1];
+        u[c] = kv8_pack(__uint_as_float(a << 16) * by,
+                        __uint_as_float(a & 0xffff0000u) * by,
+                        __uint_as_float(b << 16) * by,
+                        __uint_as_float(b & 0xffff0000u) * by);
+      }
+      if (!anew) {                         // uniform
+        if (!keep) {
+#pragma unroll
+          for (int c = 0; c < 4; c++) w[c] = kv8_again(w[c], again);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          unsigned fill = fresh ? ~0u : 0; // bytes that are new
+          if constexpr (VAL) {
+            const unsigned f = r.have >> (4 * c) & 15;
+            fill = (f & 1) * 0xffu | (f >> 1 & 1) * 0xff00u |
+                   (f >> 2 & 1) * 0xff0000u | (f >> 3) * 0xff000000u;
+          }
+          u[c] = (u[c] & fill) | (w[c] & ~fill);
+        }
+      }
+      if (fresh || anew || !keep)
+        *reinterpret_cast<uint4*>(to + place_of(i)) =
+            make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    if (lane == 0) kv_scale[2 * r.at + VAL] = now;
+  };
+  // one is loaded while the one before it is written
+  Run a, b;
+  load(a);
+  for (;;) {
+    const bool two = begins != 0;
+    if (two) load(b);
+    store(a);
+    if (!two) break;
+    const bool more = begins != 0;
+    if (more) load(a);
+    store(b);
+    if (!more) break;
   }
-  if (lane == 0) kv_scale[2 * at + val] = now;
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void kv8_write_kernel(
+    const long* __restrict__ slots, const int n_tokens, const int n_kv,
+    const int window, const unsigned n_blocks, const unsigned short* __restrict__ k,
+    const unsigned short* __restrict__ v, const long k_stride, const long v_stride,
+    float* __restrict__ kv_scale, unsigned char* __restrict__ k_cache,
+    unsigned char* __restrict__ v_cache) {
+  const int unit = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 +
+                                                  (threadIdx.x >> 6));
+  const int head = unit >> 1;
+  if (head >= n_kv) return;
+  if (unit & 1)
+    kv8_write_runs<D, true>(slots, n_tokens, n_kv, head, window, n_blocks, v, v_stride,
+                            kv_scale, v_cache);
+  else
+    kv8_write_runs<D, false>(slots, n_tokens, n_kv, head, window, n_blocks, k,
+                             k_stride, kv_scale, k_cache);
 }
 
 void launch_kv8_write(unsigned char* k_cache, unsigned char* v_cache,
                       float* kv_scale, const unsigned short* k,
                       const unsigned short* v, const long* slots, int n_tokens,
-                      int n_kv, int D, long k_stride, long v_stride,
-                      long n_slots, hipStream_t stream) {
-  if (n_tokens == 0 || n_slots == 0) return;
-  const dim3 grid((unsigned)n_tokens, (unsigned)((2 * n_kv + 3) / 4));
+                      int n_kv, int D, long k_stride, long v_stride, int n_blocks,
+                      hipStream_t stream) {
+  if (n_tokens == 0) return;
+  // at least 3000 waves, windows of at most eight
+  const long waves = 2L * n_kv * n_tokens;
+  int window = 1;
+  while (window < 8 && 2 * window * 3000L <= waves) window *= 2;
+  const dim3 grid((unsigned)((n_tokens + window - 1) / window),
+                  (unsigned)((2 * n_kv + 3) / 4));
   auto go = D == 128 ? kv8_write_kernel<128> : kv8_write_kernel<64>;
-  hipLaunchKernelGGL(go, grid, dim3(256), 0, stream, k_cache, v_cache, kv_scale, k,
-                     v, slots, n_tokens, n_kv, k_stride, v_stride, n_slots);
+  hipLaunchKernelGGL(go, grid, dim3(256), 0, stream, slots, n_tokens, n_kv, window,
+                     (unsigned)n_blocks, k, v, k_stride, v_stride, kv_scale, k_cache,
+                     v_cache);
 }
 
 }  // namespace xllm
