@@ -13,7 +13,7 @@ void launch_kv8_plan(int*, const int*, const int*, const int*, long*, long*, int
 void launch_kv8_write(unsigned char*, unsigned char*, float*, const unsigned short*,
                       const unsigned short*, const long*, int, int, int, long, long,
                       int, hipStream_t);
-int kv8_decode_parts(int, int, int);
+int kv8_decode_parts(int, int, int, int);
 void launch_kv8_decode(unsigned short*, const unsigned short*, const unsigned char*,
                        const unsigned char*, const float*, const int*, const int*,
                        float*, float*, float, int, int, int, int, int, int, long,
@@ -146,7 +146,7 @@ void attend_rows(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor kv
   }
   if (!on_bytes(q, 16)) q = q.clone(at::MemoryFormat::Contiguous);
   const int width = tables.size(1);
-  const int parts = xllm::kv8_decode_parts(S, c.n_kv, width);
+  const int parts = xllm::kv8_decode_parts(S, c.n_kv, G, width);
   Tensor ws;                                // parts, their sums, counters
   float *ws_o = nullptr, *ws_ml = nullptr;
   if (parts > 1) {
