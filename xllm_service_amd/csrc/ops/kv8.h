@@ -54,10 +54,20 @@ XLLM_DEV bf16x8 kv8_wide(unsigned lo, unsigned hi, float scale) {
   __builtin_memcpy(&y, x, 16);
   return y;
 }
-// whether one of four e4m3 values is a NaN (a byte of 0x7f but for its sign)
+// the top bits of those of four e4m3 values that are NaNs (0x7f but for the sign)
 XLLM_DEV unsigned kv8_nan(unsigned u) {
-  const unsigned x = ~u & 0x7f7f7f7fu;
-  return (x - 0x01010101u) & ~x & 0x80808080u;
+  return ~((~u & 0x7f7f7f7fu) + 0x7f7f7f7fu) & 0x80808080u;
+}
+// NaNs of 16 values become zeros; one bit each
+XLLM_DEV unsigned short kv8_drop_nan(uint4& u) {
+  unsigned bits = 0;
+  auto word = [&](unsigned& w, int at) {
+    const unsigned n = kv8_nan(w) >> 7;
+    w &= ~(n * 0xffu);
+    bits |= ((n & 1) | (n >> 7 & 2) | (n >> 14 & 4) | (n >> 21 & 8)) << at;
+  };
+  word(u.x, 0), word(u.y, 4), word(u.z, 8), word(u.w, 12);
+  return (unsigned short)bits;
 }
 // the first n of 16 bytes, zeros behind them
 XLLM_DEV uint4 kv8_first(uint4 u, int n) {

@@ -379,7 +379,10 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
   constexpr int TILE = PF_KT * D;            // elements of a K or V tile
   __shared__ __attribute__((aligned(1024))) unsigned short
       kv_lds[KG * 4 * TILE];
-  __shared__ int nan_lds[CACHE8 ? KG * 8 : 1];   // pages with a value that is none
+  // CACHE8: pages with a value that is a NaN, and which ones are, by channel
+  __shared__ int nan_on[CACHE8 ? KG * 8 : 1];
+  __shared__ __attribute__((aligned(8))) unsigned short
+      nan_at[CACHE8 ? KG * 8 * D : 1];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -548,9 +551,27 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
   auto settle = [&](int t, int buf) {
     unsigned short* dst = kv_lds + (kg * 2 + buf) * 2 * TILE;
     const int keys = min(seq_len, room) - (t * (PF_KT / PF_BS) + wid) * PF_BS;
-    // uniform: some row of the workgroup does not see all of the tile
-    const bool edge = t * PF_KT + PF_KT > ctx + pf_div(row0, by_G, sG) + 1;
-    unsigned nan = 0;
+    if (keys < PF_BS) {                          // zeros behind the last key
+#pragma unroll
+      for (int i = 0; i < N8; i++) v8[i] = kv8_first(v8[i], keys);
+    }
+    // Uniform: some row of the workgroup does not see all of the tile. A NaN there
+    // would reach it, as 0 times one is one.
+    if (t * PF_KT + PF_KT > min(ctx + pf_div(row0, by_G, sG) + 1, room)) {
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < N8; i++)
+        any |= (kv8_nan(v8[i].x) | kv8_nan(v8[i].y) | kv8_nan(v8[i].z) |
+                kv8_nan(v8[i].w)) != 0;
+      any = __any(any);
+      if (lane == 0) nan_on[(kg * 2 + buf) * 4 + wid] = any;
+      if (any) {
+#pragma unroll
+        for (int i = 0; i < N8; i++)
+          nan_at[((kg * 2 + buf) * D + lane + 64 * i) * 4 + wid] =
+              kv8_drop_nan(v8[i]);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < N8; i++) {
       const int p = lane + 64 * i;
@@ -562,19 +583,13 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
           kv8_wide(k8[i].x, k8[i].y, k8s);
       *reinterpret_cast<bf16x8*>(kr + (((c + 1) ^ xk) << 3)) =
           kv8_wide(k8[i].z, k8[i].w, k8s);
-      // values: 16 tokens of channel p; zeros behind the last key
-      const uint4 v = keys < PF_BS ? kv8_first(v8[i], keys) : v8[i];
-      if (edge) nan |= kv8_nan(v.x) | kv8_nan(v.y) | kv8_nan(v.z) | kv8_nan(v.w);
+      // values: 16 tokens of channel p
       unsigned short* vr = dst + TILE + p * PF_KT;
       const int xv = mr_swz_rows<PF_KT>(p);
       *reinterpret_cast<bf16x8*>(vr + (((2 * wid) ^ xv) << 3)) =
-          kv8_wide(v.x, v.y, v8s);
+          kv8_wide(v8[i].x, v8[i].y, v8s);
       *reinterpret_cast<bf16x8*>(vr + (((2 * wid + 1) ^ xv) << 3)) =
-          kv8_wide(v.z, v.w, v8s);
-    }
-    if (edge) {
-      const bool any = __any(nan != 0);
-      if (lane == 0) nan_lds[(kg * 2 + buf) * 4 + wid] = any;
+          kv8_wide(v8[i].z, v8[i].w, v8s);
     }
   };
 
@@ -688,37 +703,6 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
         }
       }
     // ---- O^T += V^T P^T ------------------------------------------------------
-    if constexpr (CACHE8) {
-      // A value that is a NaN counts for the rows that see it: 0 times it is one too.
-      const int* nan = nan_lds + (kg * 2 + buf) * 4;
-      if (k0 + PF_KT > wmin && (nan[0] | nan[1] | nan[2] | nan[3]) != 0) {
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++) {
-          f32x16 count = mr_zero();              // of those, by row
-#pragma unroll
-          for (int st = 0; st < 4; st++) {
-            bf16x8 a = *reinterpret_cast<const lds_bf16x8*>(
-                vt + (vbase8 ^ (st << 4)) + dt * 32 * PF_KT);
-            bf16x8 is, sees;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-              const bool none = (a[j] & 0x7fff) > 0x7f80;
-              is[j] = none ? 0x3f80 : 0;
-              a[j] = none ? (short)0 : a[j];
-              sees[j] = k0 + 16 * st + 8 * h + j < limit ? 0x3f80 : 0;
-            }
-            count = mr_mma(is, sees, count);
-#pragma unroll
-            for (int e = 0; e < TERMS; e++)
-              o_acc[dt] = mr_mma(a, p[e][st], o_acc[dt]);
-          }
-#pragma unroll
-          for (int r = 0; r < 16; r++)
-            if (count[r] > 0.0f) o_acc[dt][r] = NAN;
-        }
-        continue;
-      }
-    }
 #pragma unroll
     for (int st = 0; st < 4; st++)
 #pragma unroll
@@ -733,6 +717,22 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
         for (int e = 0; e < TERMS; e++)
           o_acc[dt] = mr_mma(a, p[e][st], o_acc[dt]);
       }
+    if constexpr (CACHE8) {
+      // values that are NaNs, zeros in the tile: for the rows that see them
+      const int* on = nan_on + (kg * 2 + buf) * 4;
+      if (k0 + PF_KT > wmin && (on[0] | on[1] | on[2] | on[3]) != 0) {
+        u64 sees = limit - k0 >= 64 ? ~0ull : (1ull << max(limit - k0, 0)) - 1;
+        for (int w = 0; w < 4; w++)
+          if (!on[w]) sees &= ~(0xffffull << (16 * w));
+        const u64* nan = reinterpret_cast<const u64*>(nan_at) + (kg * 2 + buf) * D;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+          for (int r = 0; r < 16; r++)
+            if (nan[dt * 32 + 8 * (r >> 2) + 4 * h + (r & 3)] & sees)
+              o_acc[dt][r] = NAN;
+      }
+    }
   }
 
   // ---- epilogue: o_acc[dt][r] = O[row][dt*32 + 8*(r>>2) + 4h + (r&3)] --------
