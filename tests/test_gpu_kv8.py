@@ -36,10 +36,10 @@ def ints(x, dtype=torch.int32):
     return torch.tensor(x, dtype=dtype, device=DEV)
 
 
-def filled(lens, heads, dim, seed, spare=3, big=1.0):
+def filled(lens, heads, dim, seed, spare=3, big=1.0, width=None):
     """A cache of these sequences, written by the reference on the CPU, every other
     byte of it NaN and other scales 2^60: (cache on the GPU, oracle, table)."""
-    table, pages = layout(lens, spare, seed)
+    table, pages = layout(lens, spare, seed, width)
     cache = ops.kv8_cache(pages, heads, dim)
     slots = slots_of(table, [0] * len(lens), [max(n, 0) for n in lens])
     g = torch.Generator().manual_seed(seed)
@@ -214,6 +214,70 @@ def test_prefill_of_full_steps(heads, per, dim, new, old):
     got = ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints(cu),
                                      ints(lens), dim ** -0.5)
     close(got, q, want, table, cu, lens, dim ** -0.5, 2.0 ** -8)
+
+
+# 440 to 512 workgroups of 256 rows over tables of 2048 keys and more
+LONG = [(24, 8, [600], [0]), (21, 8, [300, 400], [100, 1700]),
+        (28, 7, [513], [1600]), (64, 3, [512], [0])]
+
+
+@pytest.mark.parametrize("heads,per,new,old", LONG)
+def test_prefill_of_whole_turns(heads, per, new, old):
+    lens = [n + o for n, o in zip(new, old)]
+    cache, want, table = filled(lens, heads, 128, len(lens), width=140)
+    H, T = heads * per, sum(new)
+    q = part(rows(T + 3, H, 128, 6), H, 128)
+    cu = [sum(new[:i]) for i in range(len(new) + 1)]
+    out = torch.full((T + 3, H, 128), 7.0, dtype=torch.bfloat16, device=DEV)
+    ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints(cu), ints(lens),
+                               0.09, out=out)
+    close(out[:T], q[:T], want, table, cu, lens, 0.09, 2.0 ** -8)
+    assert (out[T:] == 7.0).all()
+    again = ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints(cu),
+                                       ints(lens), 0.09)
+    assert torch.equal(again[:T], out[:T])
+
+
+@pytest.mark.parametrize("total", [2300, 2240, 500, 300, 0, -9])
+def test_prefill_of_whole_turns_and_odd_lengths(total):
+    """A sequence longer than its table, shorter than its chunk, without keys."""
+    heads, per, T = 24, 8, 600
+    cache, want, table = filled([2240], heads, 128, 3, width=140)
+    q = part(rows(T, heads * per, 128, 6), heads * per, 128)
+    got = ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints([0, T]),
+                                     ints([total]), 0.09)
+    close(got, q, want, table, [0, T], [total], 0.09, 2.0 ** -8)
+    if total < T:
+        assert (got[:T - max(total, 0)] == 0).all()
+
+
+@pytest.mark.parametrize("token", [0, 1, 200, 255, 511])
+def test_prefill_of_whole_turns_and_values_that_are_not_finite(token):
+    heads, per, T, old = 64, 3, 512, 17
+    cache, _, table = filled([T + old], heads, 128, 3, width=140)
+    q = part(rows(T, heads * per, 128, 6), heads * per, 128)
+    at = token + old
+    cache[1].view(torch.uint8)[table[0, at // 16], :, 77, at % 16] = 0xff
+    got = ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints([0, T]),
+                                     ints([T + old]), 0.09)
+    assert got[token:, :, 77].isnan().all()
+    got[token:, :, 77] = 0.0
+    assert not got.isnan().any()
+
+
+@pytest.mark.parametrize("heads,per,dim", [(2, 4, 128), (3, 1, 64), (1, 7, 128)])
+@pytest.mark.parametrize("token", [0, 20, 63, 64, 130])
+def test_values_that_are_not_finite_anywhere(token, heads, per, dim):
+    T, old = 150, 5
+    cache, _, table = filled([T + old], heads, dim, 3)
+    q = part(rows(T, heads * per, dim, 6), heads * per, dim)
+    at = token + old
+    cache[1].view(torch.uint8)[table[0, at // 16], :, 33, at % 16] = 0xff
+    got = ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints([0, T]),
+                                     ints([T + old]), 0.09)
+    assert got[token:, :, 33].isnan().all()
+    got[token:, :, 33] = 0.0
+    assert not got.isnan().any()
 
 
 def test_rows_without_keys():

@@ -3,7 +3,7 @@
 //
 // Weights are rounded to bf16, as over bf16 pages of 128-wide heads: 2^-8 of each at
 // most, a thirty-second of what the values themselves were rounded by.
-#include "paged_rows.h"
+#include "paged_long.h"
 
 namespace xllm {
 
@@ -29,11 +29,18 @@ void launch_kv8_prefill(unsigned short* out, float* ws, const unsigned short* q,
   const PagedRows plan =
       kv8_rows(tokens, n_seqs, n_qheads / n_kv, n_kv, D, max_blocks);
   const Kv8Pages pages{reinterpret_cast<const float2*>(kv_scale), n_blocks};
+  const auto* kc = reinterpret_cast<const unsigned short*>(k_cache);
+  const auto* vc = reinterpret_cast<const unsigned short*>(v_cache);
+  if (D == 128 && plan.least == 0 && !getenv("KV8_NOLONG") &&
+      paged_long_takes(tokens, n_seqs, n_qheads / n_kv, n_kv, max_blocks)) {
+    paged_long_of<true>(out, q, kc, vc, block_tables, cu_q, seq_lens, tokens, n_seqs,
+                        scale, n_qheads, n_kv, max_blocks, q_stride, out_stride, pages,
+                        stream);
+    return;
+  }
   auto go = D == 128 ? paged_rows_of<128, 1, false, true>
                      : paged_rows_of<64, 1, false, true>;
-  go(out, ws, q, reinterpret_cast<const unsigned short*>(k_cache),
-     reinterpret_cast<const unsigned short*>(v_cache), block_tables, cu_q, seq_lens,
-     tokens, n_seqs, scale, n_qheads, n_kv, max_blocks, q_stride, out_stride, plan,
+  go(out, ws, q, kc, vc, block_tables, cu_q, seq_lens, tokens, n_seqs, scale, n_qheads, n_kv, max_blocks, q_stride, out_stride, plan,
      PagedMore{}, PagedAhead{}, pages, stream);
 }
 

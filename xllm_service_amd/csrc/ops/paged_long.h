@@ -31,6 +31,10 @@ namespace xllm {
 #define PL_ROWS 256        // rows per workgroup
 #define PL_BUFS 4          // tiles of K and V in LDS
 
+// CACHE8: pages of 8 bits (kv8.h), as in paged_rows.h: among its products a wave converts
+// its page of two steps later, as values are read from the half step before their bundle
+// on, and asks for the one after it.
+template <bool CACHE8>
 __global__ __launch_bounds__(512) void paged_attn_long_kernel(
     unsigned short* __restrict__ out,        // [total_q, n_qheads, D]
     const unsigned short* __restrict__ q,    // [total_q, n_qheads, D] bf16
@@ -40,7 +44,8 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
     const int* __restrict__ cu_q,            // [num_seqs+1] query offsets
     const int* __restrict__ seq_lens,        // [num_seqs] total key len
     const int n_seqs, const float scale, const int G, const int n_kv,
-    const int max_blocks, const long q_stride, const long out_stride) {
+    const int max_blocks, const long q_stride, const long out_stride,
+    const Kv8Pages c8) {
   constexpr int D = 128;
   constexpr int KS = D / 16;                 // k steps of a score product
   constexpr int DT = D / 32;                 // 32-wide tiles of the head
@@ -50,6 +55,10 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
   constexpr int TILE = PF_KT * D;            // elements of a K or V tile
   __shared__ __attribute__((aligned(1024))) unsigned short
       kv_lds[2 * PL_BUFS * TILE];
+  // CACHE8: pages with a value that is a NaN, and which ones are, by channel
+  __shared__ int nan_on[CACHE8 ? PL_BUFS * 4 : 1];
+  __shared__ __attribute__((aligned(8))) unsigned short
+      nan_at[CACHE8 ? PL_BUFS * D * 4 : 1];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -65,9 +74,11 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
             q_len = place.q_len, seq_len = place.seq_len;
   const int ctx = seq_len - q_len;
   const int rows = q_len * G;
+  // a table that ends before its sequence: what it does not have is not seen
+  const int room = CACHE8 ? max_blocks * PF_BS : INT_MAX;
 
   const int row0 = lt * PL_ROWS;
-  const int kmax = ctx + (min(row0 + PL_ROWS, rows) - 1) / G + 1;
+  const int kmax = min(ctx + (min(row0 + PL_ROWS, rows) - 1) / G + 1, room);
   const int n = (max(kmax, 0) + PF_KT - 1) / PF_KT;   // tiles; rows without keys: 0
 
   // ---- this lane's row -----------------------------------------------------
@@ -77,9 +88,9 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
   const bool row_ok = rho < rows;
   const int qi = rho / G;
   const int head = kvh * G + rho - qi * G;
-  const int limit = row_ok ? ctx + qi + 1 : 0;   // keys this row sees
-  const int wmin = ctx + wrow0 / G + 1;          // fewest of a row in the wave
-  const int wmax = ctx + (min(wrow0 + 32, rows) - 1) / G + 1;
+  const int limit = row_ok ? min(ctx + qi + 1, room) : 0;   // keys this row sees
+  const int wmin = min(ctx + wrow0 / G + 1, room);   // fewest of a row in the wave
+  const int wmax = min(ctx + (min(wrow0 + 32, rows) - 1) / G + 1, room);
 
   const PagedScore sc = paged_score<false>(PagedMore{}, scale, 0);
   // rows past the last one hold its query: their results go nowhere
@@ -98,7 +109,7 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
   // ---- staging: waves 0-3 move a page of K each, waves 4-7 one of V ----------
   const int half = wid >> 2, page4 = wid & 3;
   const int* btab = block_tables + (long)seq * max_blocks;
-  const int last_blk = (seq_len - 1) / PF_BS;
+  const int last_blk = (min(seq_len, room) - 1) / PF_BS;
   const int srow = lane / CPR, spos = lane % CPR;
   const unsigned short* cache = half ? v_cache : k_cache;
   // byte offset in a page of what this lane moves: row r of the page, its
@@ -115,10 +126,25 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
   // is keys, one tile per lane: what is left to do per tile is three v_readlane. A
   // row past the last key, and a tile past the last one, is out of the bounds.
   int tb = 0;
-  unsigned from_lo = 0, from_hi = 0, bytes = 0;
+  unsigned from_lo = 0, from_hi = 0, bytes = 0, size = 0;
   auto look_up = [&]() {
     const int t = tb + lane,
               pg = max(min(t, n - 1), 0) * (PF_KT / PF_BS) + page4;
+    if constexpr (CACHE8) {
+      const bool there = t < n && pg <= last_blk;
+      int id = there ? btab[pg] : 0;             // an id of no page is page 0
+      id = (unsigned)id < (unsigned)c8.blocks ? id : 0;
+      const long of = (long)id * n_kv + kvh;
+      const unsigned long long at = (unsigned long long)(
+          reinterpret_cast<const char*>(cache) + of * (PF_BS * D));
+      from_lo = (unsigned)at;
+      from_hi = (unsigned)(at >> 32);
+      bytes = there ? PF_BS * D : 0;
+      const float2 both = c8.scale[of];
+      size = __float_as_uint(half ? both.y : both.x);
+      asm volatile("" : "+v"(from_lo), "+v"(from_hi), "+v"(bytes), "+v"(size));
+      return;
+    }
     const long id = btab[min(pg, last_blk)];
     const unsigned long long at = (unsigned long long)(
         cache + (id * n_kv + kvh) * (PF_BS * D));
@@ -140,6 +166,61 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
 #pragma unroll
     for (int k = 0; k < NI; k++) mr_to_lds(src, off[k], dst + k * RPI * D);
   };
+  // 8 bits: this wave's page of bundle j to registers, 16 B a lane, ...
+  uint4 page8[2];
+  float scale8 = 0.0f;
+  auto fetch8 = [&](unsigned j) {
+    const int i = (int)j - half - tb;
+    const unsigned lo = __builtin_amdgcn_readlane(from_lo, i);
+    const unsigned hi = __builtin_amdgcn_readlane(from_hi, i);
+    const auto src = mr_buffer((const void*)((unsigned long long)hi << 32 | lo),
+                               __builtin_amdgcn_readlane(bytes, i));
+    page8[0] = mr_load(src, lane * 16);
+    page8[1] = mr_load(src, lane * 16 + 1024);
+    scale8 = __uint_as_float(__builtin_amdgcn_readlane(size, i));
+  };
+  // ... and from there to its buffer: keys, chunk p / 16 of 16 channels of token p % 16;
+  // values, 16 tokens of channel p; p the lane, and 64 more
+  const int to8 = half ? lane * PF_KT + (((2 * page4) ^ mr_swz_rows<PF_KT>(lane)) << 3)
+                       : (page4 * PF_BS + (lane & 15)) * D +
+                             (((lane >> 4 << 1) ^ mr_swz_rows<D>(lane & 15)) << 3);
+  const int more8 = half ? 64 * PF_KT : 64;
+  const int least8 = min(ctx + row0 / G + 1, room);   // fewest keys of a row of all
+  auto convert8 = [&](unsigned j) {
+    if (half) {
+      const int t = (int)j - 1;
+      const int keys = min(seq_len, room) - t * PF_KT - page4 * PF_BS;
+      if (keys < PF_BS) {                        // zeros behind the last key
+        page8[0] = kv8_first(page8[0], keys);
+        page8[1] = kv8_first(page8[1], keys);
+      }
+      // uniform: some row of the workgroup does not see all of the tile
+      if (t * PF_KT + PF_KT > least8) {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+          any |= (kv8_nan(page8[i].x) | kv8_nan(page8[i].y) | kv8_nan(page8[i].z) |
+                  kv8_nan(page8[i].w)) != 0;
+        any = __any(any);
+        if (lane == 0) nan_on[j % PL_BUFS * 4 + page4] = any;
+        if (any) {
+#pragma unroll
+          for (int i = 0; i < 2; i++)
+            nan_at[(j % PL_BUFS * D + lane + 64 * i) * 4 + page4] =
+                kv8_drop_nan(page8[i]);
+        }
+      }
+    }
+    lds_u16* dst = (lds_u16*)kv_lds + (j % PL_BUFS * 2 + half) * TILE;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int at = i ? to8 ^ more8 : to8;
+      *reinterpret_cast<lds_bf16x8*>(dst + at) =
+          kv8_wide(page8[i].x, page8[i].y, scale8);
+      *reinterpret_cast<lds_bf16x8*>(dst + (at ^ 8)) =
+          kv8_wide(page8[i].z, page8[i].w, scale8);
+    }
+  };
   // before bundle j is staged
   auto ready = [&](unsigned j) {
     if ((int)j - half - tb < 64) return;
@@ -149,14 +230,20 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
   // A half step ends. `later` bundles of this wave may be on the way
   auto meet = [&](int later) {
     __builtin_amdgcn_sched_barrier(0);
-    if (later == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NI) : "memory");
-    else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI) : "memory");
+    // (8 bits: what a wave has written lies before reads of its own that it has
+    // waited for)
+    if constexpr (CACHE8) asm volatile("" ::: "memory");
+    else if (later == 2)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NI) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
 
   const int kbase = mr_row_base<D>(lane), vbase = mr_col_base<D>(lane);
+  const int vbase8 = c32 * PF_KT + ((h ^ mr_swz_rows<PF_KT>(c32)) << 3);
   const float c = sc.c;
   f32x16 s[2];
   bf16x8 p[4];
@@ -175,8 +262,13 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
   // operands of four products: 16 values' rows, or two steps of the keys'
   auto fetch_v = [&](bf16x8 (&f)[DT], const lds_u16* vt, int st) {
 #pragma unroll
-    for (int dt = 0; dt < DT; dt++)
-      f[dt] = mr_cols_own<D>(vt + (vbase ^ (dt << 5)) + st * 16 * D);
+    for (int dt = 0; dt < DT; dt++) {
+      if constexpr (CACHE8)
+        f[dt] = *reinterpret_cast<const lds_bf16x8*>(vt + (vbase8 ^ (st << 4)) +
+                                                     dt * 32 * PF_KT);
+      else
+        f[dt] = mr_cols_own<D>(vt + (vbase ^ (dt << 5)) + st * 16 * D);
+    }
   };
   auto fetch_k = [&](bf16x8 (&f)[4], const lds_u16* kt, int ks) {
 #pragma unroll
@@ -244,16 +336,58 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
     }
   };
 
+  // values of tile t that are NaNs, zeros in its buffer: for the rows that see them
+  auto nans = [&](int t) {
+    if constexpr (CACHE8) {
+      const int buf = (t + 1) % PL_BUFS, k0 = t * PF_KT;
+      if (k0 + PF_KT <= least8) return;          // uniform
+      const int* on = nan_on + buf * 4;
+      if ((on[0] | on[1] | on[2] | on[3]) == 0) return;
+      unsigned long long sees =
+          limit - k0 >= 64 ? ~0ull : (1ull << max(limit - k0, 0)) - 1;
+      for (int w = 0; w < 4; w++)
+        if (!on[w]) sees &= ~(0xffffull << (16 * w));
+      const auto* nan = reinterpret_cast<const unsigned long long*>(nan_at) + buf * D;
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          if (nan[dt * 32 + 8 * (r >> 2) + 4 * h + (r & 3)] & sees)
+            o_acc[dt][r] = NAN;
+    }
+  };
+
   // tiles with keys that this wave's rows see
   const unsigned mine =
       wave_on ? (unsigned)(max(wmax, 0) + PF_KT - 1) / PF_KT : 0;
   look_up();
+  if constexpr (CACHE8) {
+    if (!half) {
+      fetch8(0);
+      convert8(0);
+    }
+    fetch8(1);
+    convert8(1);
+    fetch8(2);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  } else {
 #pragma unroll
-  for (int i = 0; i < PL_BUFS - 1; i++)
-    if (i > 0 || !half) stage(i);
+    for (int i = 0; i < PL_BUFS - 1; i++)
+      if (i > 0 || !half) stage(i);
+  }
   if (half) meet(2);
   unsigned j = 0;
   const lds_u16 *kt, *vt;                      // of bundle j; values of the next
+  // a step's share of the loads
+  auto move = [&]() {
+    if constexpr (CACHE8) {
+      // what is read from the half step before bundle j + 2 on
+      convert8(j + 2);
+      fetch8(j + 3);
+    } else {
+      stage(j + PL_BUFS - 1);
+    }
+  };
   auto open = [&]() {
     ready(j + PL_BUFS - 1);
     meet(1);
@@ -265,7 +399,7 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
     bf16x8 f[DT], g[DT], fk[4];
     open();
     fetch_k(fk, kt, 0);
-    stage(j + PL_BUFS - 1);
+    move();
     all_scores(fk, kt);
     __builtin_amdgcn_s_setprio(0);
     for (;;) {
@@ -284,28 +418,31 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
       __builtin_amdgcn_sched_barrier(0);
       fetch_v(g, v, 3);
       values(f, 2);
-      stage(j + PL_BUFS - 1);
+      move();
       __builtin_amdgcn_sched_barrier(0);
       fetch_k(fk, kt, 0);
       values(g, 3);
+      nans((int)j - 1);
       __builtin_amdgcn_sched_barrier(0);
       all_scores(fk, kt);
       __builtin_amdgcn_s_setprio(0);
     }
-    stage(j + PL_BUFS - 1);
+    move();
     values(f, 0);
 #pragma unroll
     for (int st = 1; st < 4; st++) {
       fetch_v(f, kt + TILE, st);
       values(f, st);
     }
+    nans((int)j - 1);
     __builtin_amdgcn_s_setprio(0);
     if ((int)j < n) meet(2);
     j++;
   }
   for (; (int)j <= n; j++) {
     open();
-    stage(j + PL_BUFS - 1);
+    move();
+    if constexpr (CACHE8) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_setprio(0);
     if ((int)j < n) meet(2);
   }
@@ -357,6 +494,22 @@ inline bool paged_long_takes(long tokens, int n_seqs, int G, int n_kv,
   return n_seqs > 1 || 2 * keys >= 3 * tokens || keys >= 6144;
 }
 
+template <bool CACHE8>
+inline void paged_long_of(unsigned short* out, const unsigned short* q,
+                          const unsigned short* k_cache,
+                          const unsigned short* v_cache, const int* block_tables,
+                          const int* cu_q, const int* seq_lens, long tokens,
+                          int n_seqs, float scale, int n_qheads, int n_kv,
+                          int max_blocks, long q_stride, long out_stride,
+                          const Kv8Pages& c8, hipStream_t stream) {
+  const int G = n_qheads / n_kv;
+  if (tokens == 0 || n_seqs <= 0) return;
+  hipLaunchKernelGGL(
+      paged_attn_long_kernel<CACHE8>,
+      dim3((unsigned)(paged_rows_tiles<PL_ROWS>(tokens, n_seqs, G) * n_kv)),
+      dim3(512), 0, stream, out, q, k_cache, v_cache, block_tables, cu_q,
+      seq_lens, n_seqs, scale, G, n_kv, max_blocks, q_stride, out_stride, c8);
+}
 inline void paged_long(unsigned short* out, const unsigned short* q,
                        const unsigned short* k_cache,
                        const unsigned short* v_cache, const int* block_tables,
@@ -364,13 +517,9 @@ inline void paged_long(unsigned short* out, const unsigned short* q,
                        int n_seqs, float scale, int n_qheads, int n_kv,
                        int max_blocks, long q_stride, long out_stride,
                        hipStream_t stream) {
-  const int G = n_qheads / n_kv;
-  if (tokens == 0 || n_seqs <= 0) return;
-  hipLaunchKernelGGL(
-      paged_attn_long_kernel,
-      dim3((unsigned)(paged_rows_tiles<PL_ROWS>(tokens, n_seqs, G) * n_kv)),
-      dim3(512), 0, stream, out, q, k_cache, v_cache, block_tables, cu_q,
-      seq_lens, n_seqs, scale, G, n_kv, max_blocks, q_stride, out_stride);
+  paged_long_of<false>(out, q, k_cache, v_cache, block_tables, cu_q, seq_lens, tokens,
+                       n_seqs, scale, n_qheads, n_kv, max_blocks, q_stride,
+                       out_stride, Kv8Pages{}, stream);
 }
 
 }  // namespace xllm

@@ -547,6 +547,8 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
           reinterpret_cast<const char*>(v_cache) + from + i * 1024);
     }
   };
+  const int least8 =                             // fewest keys of a row of all
+      min(ctx + pf_div(row0, by_G, sG) + 1, room);
   // ... and from there to their tile
   auto settle = [&](int t, int buf) {
     unsigned short* dst = kv_lds + (kg * 2 + buf) * 2 * TILE;
@@ -557,7 +559,7 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
     }
     // Uniform: some row of the workgroup does not see all of the tile. A NaN there
     // would reach it, as 0 times one is one.
-    if (t * PF_KT + PF_KT > min(ctx + pf_div(row0, by_G, sG) + 1, room)) {
+    if (t * PF_KT + PF_KT > least8) {
       bool any = false;
 #pragma unroll
       for (int i = 0; i < N8; i++)
@@ -720,7 +722,7 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
     if constexpr (CACHE8) {
       // values that are NaNs, zeros in the tile: for the rows that see them
       const int* on = nan_on + (kg * 2 + buf) * 4;
-      if (k0 + PF_KT > wmin && (on[0] | on[1] | on[2] | on[3]) != 0) {
+      if (k0 + PF_KT > least8 && (on[0] | on[1] | on[2] | on[3]) != 0) {
         u64 sees = limit - k0 >= 64 ? ~0ull : (1ull << max(limit - k0, 0)) - 1;
         for (int w = 0; w < 4; w++)
           if (!on[w]) sees &= ~(0xffffull << (16 * w));
