@@ -216,9 +216,10 @@ def test_prefill_of_full_steps(heads, per, dim, new, old):
     close(got, q, want, table, cu, lens, dim ** -0.5, 2.0 ** -8)
 
 
-# 440 to 512 workgroups of 256 rows over tables of 2048 keys and more
+# 440 to 512 workgroups of 256 rows, and fewer behind longer contexts
 LONG = [(24, 8, [600], [0]), (21, 8, [300, 400], [100, 1700]),
-        (28, 7, [513], [1600]), (64, 3, [512], [0])]
+        (28, 7, [513], [1600]), (64, 3, [512], [0]),
+        (32, 4, [300, 270], [1900, 30]), (65, 1, [900], [200])]
 
 
 @pytest.mark.parametrize("heads,per,new,old", LONG)

@@ -7,6 +7,22 @@
 
 namespace xllm {
 
+// Where paged_long.h takes less time: there a page is converted once for 256 rows, not
+// 128, so earlier than with bf16 pages. By workgroups of 256 rows and the keys that a row
+// sees on average, were the prompts equal. 170 drawn batches, time over that of
+// paged_rows.h: from 440 workgroups on, over 550 keys 0.77 to 0.99 (0.88), 250 to 550 0.94
+// to 1.09, fewer 1.02 to 1.17; 300 to 440, from 1200 keys on 0.79 to 0.96 (0.88), fewer 0.93
+// to 1.17; 256 to 300, from 2500 on 0.85 to 1.05, fewer 0.98 to 1.30; below 1.0 to 1.4.
+// Prompts of few rows leave most of 256 idle: 60 sequences of 160 rows over 2000 keys
+// 0.72, 64 of 120 0.91, of 48 1.06, 128 of 16 1.18.
+static bool kv8_long_takes(long tokens, int n_seqs, int G, int n_kv, int D,
+                           long max_blocks) {
+  if (D != 128 || tokens * G < 120L * n_seqs) return false;
+  const long each = (tokens * G + n_seqs * (long)PL_ROWS - 1) / (n_seqs * (long)PL_ROWS);
+  const long wgs = each * n_seqs * n_kv;
+  const long sees = max_blocks * PF_BS - tokens / n_seqs / 2;
+  return wgs >= 440 ? sees >= 550 : wgs >= 300 ? sees >= 1200 : wgs >= 256 && sees >= 2500;
+}
 static PagedRows kv8_rows(long tokens, int n_seqs, int G, int n_kv, int D,
                           int max_blocks) {
   return paged_rows_plan(tokens, n_seqs, G, n_kv, D, max_blocks, 1, false);
@@ -14,7 +30,9 @@ static PagedRows kv8_rows(long tokens, int n_seqs, int G, int n_kv, int D,
 // floats of scratch that a call asks for
 long kv8_prefill_scratch(long tokens, int n_seqs, int G, int n_kv, int D,
                          int max_blocks) {
-  if (tokens == 0 || n_seqs <= 0) return 0;
+  if (tokens == 0 || n_seqs <= 0 ||
+      kv8_long_takes(tokens, n_seqs, G, n_kv, D, max_blocks))
+    return 0;
   return kv8_rows(tokens, n_seqs, G, n_kv, D, max_blocks).scratch;
 }
 
@@ -26,18 +44,17 @@ void launch_kv8_prefill(unsigned short* out, float* ws, const unsigned short* q,
                         int max_blocks, int n_blocks, long q_stride,
                         long out_stride, hipStream_t stream) {
   if (tokens == 0 || n_seqs <= 0) return;
-  const PagedRows plan =
-      kv8_rows(tokens, n_seqs, n_qheads / n_kv, n_kv, D, max_blocks);
   const Kv8Pages pages{reinterpret_cast<const float2*>(kv_scale), n_blocks};
   const auto* kc = reinterpret_cast<const unsigned short*>(k_cache);
   const auto* vc = reinterpret_cast<const unsigned short*>(v_cache);
-  if (D == 128 && plan.least == 0 && !getenv("KV8_NOLONG") &&
-      paged_long_takes(tokens, n_seqs, n_qheads / n_kv, n_kv, max_blocks)) {
+  if (kv8_long_takes(tokens, n_seqs, n_qheads / n_kv, n_kv, D, max_blocks)) {
     paged_long_of<true>(out, q, kc, vc, block_tables, cu_q, seq_lens, tokens, n_seqs,
                         scale, n_qheads, n_kv, max_blocks, q_stride, out_stride, pages,
                         stream);
     return;
   }
+  const PagedRows plan =
+      kv8_rows(tokens, n_seqs, n_qheads / n_kv, n_kv, D, max_blocks);
   auto go = D == 128 ? paged_rows_of<128, 1, false, true>
                      : paged_rows_of<64, 1, false, true>;
   go(out, ws, q, kc, vc, block_tables, cu_q, seq_lens, tokens, n_seqs, scale, n_qheads, n_kv, max_blocks, q_stride, out_stride, plan,
