@@ -267,10 +267,11 @@ def test_prefill_of_whole_turns_and_values_that_are_not_finite(token):
 
 
 @pytest.mark.parametrize("heads,per,dim", [(2, 4, 128), (3, 1, 64), (1, 7, 128)])
+@pytest.mark.parametrize("width", [10, 400])
 @pytest.mark.parametrize("token", [0, 20, 63, 64, 130])
-def test_values_that_are_not_finite_anywhere(token, heads, per, dim):
+def test_values_that_are_not_finite_anywhere(token, heads, per, dim, width):
     T, old = 150, 5
-    cache, _, table = filled([T + old], heads, dim, 3)
+    cache, _, table = filled([T + old], heads, dim, 3, width=width)
     q = part(rows(T, heads * per, dim, 6), heads * per, dim)
     at = token + old
     cache[1].view(torch.uint8)[table[0, at // 16], :, 33, at % 16] = 0xff
@@ -279,6 +280,42 @@ def test_values_that_are_not_finite_anywhere(token, heads, per, dim):
     assert got[token:, :, 33].isnan().all()
     got[token:, :, 33] = 0.0
     assert not got.isnan().any()
+
+
+# few rows over wide tables, whose keys are split over workgroups, and many over few keys
+ROWS = [(2, 4, 128, [9], [1200], 300), (2, 4, 128, [40, 3], [700, 90], 400),
+        (1, 8, 64, [30], [900], 260), (16, 4, 128, [80] * 9, [0] * 9, 8),
+        (16, 4, 128, [300, 7], [20, 0], 21), (12, 3, 64, [70] * 14, [3] * 14, 6),
+        (4, 4, 128, [600], [300], 600), (2, 5, 128, [11, 300, 1], [0, 5, 900], 700)]
+
+
+@pytest.mark.parametrize("heads,per,dim,new,old,width", ROWS)
+def test_prefill_by_tables(heads, per, dim, new, old, width):
+    lens = [n + o for n, o in zip(new, old)]
+    cache, want, table = filled(lens, heads, dim, len(lens), width=width)
+    H, T = heads * per, sum(new)
+    q = part(rows(T + 3, H, dim, 6), H, dim)
+    cu = [sum(new[:i]) for i in range(len(new) + 1)]
+    out = torch.full((T + 3, H, dim), 7.0, dtype=torch.bfloat16, device=DEV)
+    ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints(cu), ints(lens),
+                               dim ** -0.5, out=out)
+    close(out[:T], q[:T], want, table, cu, lens, dim ** -0.5, 2.0 ** -8)
+    assert (out[T:] == 7.0).all()
+
+
+@pytest.mark.parametrize("heads,per,dim,width", [(2, 4, 128, 12), (3, 1, 64, 12),
+                                                 (2, 4, 128, 400), (3, 1, 64, 400)])
+@pytest.mark.parametrize("total", [400, 150, 60, 0, -9])
+def test_prefill_and_odd_lengths(total, heads, per, dim, width):
+    """A sequence longer than its table, shorter than its chunk, without keys."""
+    T = 100
+    cache, want, table = filled([192], heads, dim, 3, width=width)
+    q = part(rows(T, heads * per, dim, 6), heads * per, dim)
+    if width > 12:
+        table = table[:, :12].repeat(1, -(-width // 12))[:, :width]
+    got = ops.paged_attn_prefill_kv8(q, *cache, table.contiguous().to(DEV),
+                                     ints([0, T]), ints([total]), 0.09)
+    close(got, q, want, table, [0, T], [total], 0.09, 2.0 ** -8)
 
 
 def test_rows_without_keys():

@@ -3,9 +3,27 @@
 //
 // Weights are rounded to bf16, as over bf16 pages of 128-wide heads: 2^-8 of each at
 // most, a thirty-second of what the values themselves were rounded by.
+#include "kv8_short.h"
 #include "paged_long.h"
 
 namespace xllm {
+
+// Where kv8_short.h takes less time than paged_rows.h: one turn of its workgroups, two to
+// a CU (three, 64 wide), and over long tables up to 1400 of them. A few of them over many
+// keys go to the other kernel, which splits keys over workgroups, evenly those of a single
+// sequence. 240 drawn batches, time over that of paged_rows.h: in one turn, up to so many
+// keys, 0.40 to 1.18 (0.75), past them 0.76 to 2.1; more workgroups over enough keys 0.71 to
+// 1.08 (0.90), over fewer 0.86 to 1.32. Us, paged_rows.h | here | bf16 pages: 300 tokens of
+// 32/8 heads 15.0 | 9.8 | 12.8, 3 x 61-333 behind 0.5-3 k of 28/4 29.4 | 23.4 | 26.9, 100
+// behind 800 28 | 11.7 | 14, 8 x 64-448 of 12/12 of 64 12.0 | 11.6 | 13.5.
+static bool kv8_short_takes(long tokens, int n_seqs, int G, int n_kv, int D,
+                            long max_blocks) {
+  const long wgs = paged_rows_tiles<K8S_ROWS>(tokens, n_seqs, G) * n_kv;
+  const long keys = max_blocks * PF_BS;
+  if (wgs <= (D == 64 ? 768 : 512))
+    return keys <= 1536 + (n_seqs == 1 ? 8 : 16) * wgs;
+  return wgs <= 1400 && keys >= (D == 64 ? 700 : wgs <= 1024 ? 400 : 1000);
+}
 
 // Where paged_long.h takes less time: there a page is converted once for 256 rows, not
 // 128, so earlier than with bf16 pages. By workgroups of 256 rows and the keys that a row
@@ -31,6 +49,7 @@ static PagedRows kv8_rows(long tokens, int n_seqs, int G, int n_kv, int D,
 long kv8_prefill_scratch(long tokens, int n_seqs, int G, int n_kv, int D,
                          int max_blocks) {
   if (tokens == 0 || n_seqs <= 0 ||
+      kv8_short_takes(tokens, n_seqs, G, n_kv, D, max_blocks) ||
       kv8_long_takes(tokens, n_seqs, G, n_kv, D, max_blocks))
     return 0;
   return kv8_rows(tokens, n_seqs, G, n_kv, D, max_blocks).scratch;
@@ -45,6 +64,12 @@ void launch_kv8_prefill(unsigned short* out, float* ws, const unsigned short* q,
                         long out_stride, hipStream_t stream) {
   if (tokens == 0 || n_seqs <= 0) return;
   const Kv8Pages pages{reinterpret_cast<const float2*>(kv_scale), n_blocks};
+  if (kv8_short_takes(tokens, n_seqs, n_qheads / n_kv, n_kv, D, max_blocks)) {
+    auto go = D == 128 ? kv8_short<128> : kv8_short<64>;
+    go(out, q, k_cache, v_cache, block_tables, cu_q, seq_lens, tokens, n_seqs, scale,
+       n_qheads, n_kv, max_blocks, q_stride, out_stride, pages, stream);
+    return;
+  }
   const auto* kc = reinterpret_cast<const unsigned short*>(k_cache);
   const auto* vc = reinterpret_cast<const unsigned short*>(v_cache);
   if (kv8_long_takes(tokens, n_seqs, n_qheads / n_kv, n_kv, D, max_blocks)) {
