@@ -465,6 +465,7 @@ def test_a_run_of_them():
         lens = new
 
 
+@torch.inference_mode()                       # as the engine's graphs are captured
 def test_captured_steps():
     """Two captured steps that share a pool, replayed by turns with eager work
     between them: each replay is the eager result. Rows of padding have no slot."""
@@ -577,3 +578,28 @@ def test_refusals():
     no(e, tab, lens.cpu(), lens, lens, 4)
     no(e, tab, lens, lens, lens, -1)
     no(e, tab.expand(4, 3), lens, lens, lens, 4)
+
+
+@pytest.mark.parametrize("model", ["llama-tiny", "llama-debug-128", "opt-125m"])
+def test_engine(model):
+    """The engine over 8-bit pages: captured decode steps are the eager ones."""
+    from xllm_service_amd.engine.engine import LLMEngine
+    from xllm_service_amd.engine.sampling import SamplingParams
+    prompts = [[5, 9, 2, 7] * 30, [3], list(range(40, 100))]
+    sp = SamplingParams(max_tokens=20, ignore_eos=True)
+    outs = []
+    for graphs in (False, True):
+        eng = LLMEngine(model, device="cuda:0", max_kv_blocks=64, seed=3,
+                        max_num_seqs=4, max_batched_tokens=64, max_model_len=256,
+                        enable_graphs=graphs, kv_cache_dtype="fp8")
+        assert (eng.runner.graph_runner is not None) == graphs
+        outs.append(eng.generate(prompts, sp))
+        assert [len(o) for o in outs[-1]] == [20] * 3
+        assert all(c[2].isfinite().all() for c in eng.runner.kv_caches)
+        moved = eng.import_block_bytes([5], eng.export_block_bytes([1]))
+        assert moved is None
+        for c in eng.runner.paged_tensors():
+            assert torch.equal(c[5], c[1])
+        del eng
+        torch.cuda.empty_cache()
+    assert outs[0] == outs[1]

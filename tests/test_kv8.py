@@ -180,3 +180,78 @@ def test_refusals():
     no(p, x, k8, v8, s, tab, cu.long(), lens, 1.0)
     no(p, x, k8, v8, s, tab[:0], cu, lens, 1.0)
     no(p, x, k8, v8, s[:2], tab, cu, lens, 1.0)
+
+
+# ---- the engine over such a cache --------------------------------------------
+def engine(model="llama-tiny", **kw):
+    from xllm_service_amd.engine.engine import LLMEngine
+    return LLMEngine(model, device="cpu", seed=3, max_num_seqs=4, **kw)
+
+
+PROMPTS = [[5, 9, 2, 7] * 9, [3], list(range(40, 75))]
+
+
+@pytest.mark.parametrize("model", ["llama-tiny", "opt-125m"])
+def test_engine(model):
+    """Prompts in chunks and tokens behind them, pages that are shared, and blocks
+    that move as bytes."""
+    from xllm_service_amd.engine.sampling import SamplingParams
+    sp = SamplingParams(max_tokens=6, ignore_eos=True)
+    eng = engine(model, max_kv_blocks=40, kv_cache_dtype="fp8",
+                 max_batched_tokens=16)
+    out = eng.generate(PROMPTS, sp)
+    assert [len(o) for o in out] == [6] * 3
+    assert eng.generate(PROMPTS, sp) == out          # over pages of before
+    assert all(len(c) == 3 for c in eng.runner.kv_caches)
+    other = engine(model, max_kv_blocks=40, kv_cache_dtype="fp8")
+    other.import_block_bytes([4, 2], eng.export_block_bytes([0, 1]))
+    for a, b in zip(eng.runner.paged_tensors(), other.runner.paged_tensors()):
+        assert torch.equal(a[:2].view(torch.uint8), b[[4, 2]].view(torch.uint8))
+    with pytest.raises(ValueError):
+        engine(model, max_kv_blocks=8).import_block_bytes(
+            [0], eng.export_block_bytes([0]))
+
+
+def test_engine_first_logits():
+    """Logits over 8-bit pages are near those over 32-bit ones: values are off by
+    2^-4 of themselves at most, and what attention adds to a row by as much of the
+    sum of their sizes."""
+    from xllm_service_amd.engine.metadata import AttnMetadata
+    outs = []
+    for kind in (None, "fp8"):
+        eng = engine(max_kv_blocks=8, kv_cache_dtype=kind)
+        T = 37
+        meta = AttnMetadata(
+            T, 0, torch.arange(T), cu_q=torch.tensor([0, T]).int(),
+            prefill_seq_lens=torch.tensor([T]).int(),
+            prefill_block_tables=torch.arange(3).int()[None])
+        attn = eng.model.layers[0].attn
+        x = torch.randn(T, eng.cfg.hidden_size,
+                        generator=torch.Generator().manual_seed(1))
+        attn.o_proj = torch.nn.Identity()
+        with torch.inference_mode():
+            outs.append(attn(x, torch.arange(T), eng.runner.kv_caches[0], meta,
+                             eng.model.cos_sin))
+            kv = attn.qkv_proj(x)
+    heads = eng.cfg.num_kv_heads * eng.cfg.head_dim
+    k, v = kv[:, -2 * heads:-heads], kv[:, -heads:]
+    q = kv[:, :-2 * heads]
+    # a score moves by at most 2^-4 |q| |k| (and the least step of a page)
+    off = 2.0 ** -4 * q.unflatten(1, (-1, 64)).norm(dim=-1).max() \
+        * k.unflatten(1, (-1, 64)).norm(dim=-1).max() / 8
+    bound = (2.0 ** -4 + 2 * off) * v.abs().max() + 2.0 ** -9 * v.abs().max()
+    diff = (outs[0] - outs[1]).abs().max()
+    assert 0 < diff < bound
+
+
+def test_engine_holds_twice_the_blocks_and_refuses():
+    from xllm_service_amd.engine.cache_spec import default_specs
+    from xllm_service_amd.models.config import get_config
+    cfg = get_config("llama-3-8b")
+    two = [sum(s.block_bytes(16, 2) for s in default_specs(cfg, 8, kind))
+           for kind in (None, "fp8")]
+    assert 1.98 < two[0] / two[1] <= 2.0
+    for model, kind in (("llama-tiny", "int8"), ("qwen2-vl-tiny", "fp8"),
+                        ("zokanex-tiny", "fp8")):
+        with pytest.raises(ValueError):
+            engine(model, max_kv_blocks=8, kv_cache_dtype=kind)

@@ -122,6 +122,7 @@ int check_attention(const Tensor& out, const Tensor& q, const Cache& c,
               "kv8: out must have the shape of q, and a place for each row");
   TORCH_CHECK(q.size(1) > 0 && q.size(1) % c.n_kv == 0,
               "kv8: query heads must be a multiple of the cache's");
+  TORCH_CHECK(q.size(0) * q.size(1) < (1L << 27), "kv8: too many rows");
   return (int)(q.size(1) / c.n_kv);
 }
 

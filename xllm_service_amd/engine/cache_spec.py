@@ -7,6 +7,8 @@ runner allocates the tensors and hands layer i its entry of `kv_caches`:
                    value cache has v_dim in place of head_dim when given;
                    with values_are_keys there is one tensor, handed out as
                    both members of the pair)
+  PagedKV8         (k_cache, v_cache, kv_scale) in 8 bits with a scale for each
+                   block and head (ops.kv8_cache)
   PagedLatent      one tensor [blocks, block, width] (a shared row per token)
   RecurrentState   one fp32 tensor [state_slots, heads, dim, vdim]; a
                    sequence owns one slot for its whole life
@@ -16,7 +18,8 @@ runner allocates the tensors and hands layer i its entry of `kv_caches`:
   CacheGroup       a tuple of the above for a layer that keeps several things
                    (its entry of `kv_caches` is the tuple of their tensors)
 
-Models without `cache_specs()` get PagedKV for every layer.
+Models without `cache_specs()` get PagedKV for every layer, or PagedKV8 where the
+engine is asked for an 8-bit cache.
 """
 from __future__ import annotations
 
@@ -39,6 +42,16 @@ class PagedKV:
         per_token = self.head_dim + (0 if self.values_are_keys
                                      else self.value_dim)
         return self.n_kv * block_size * per_token * dtype_bytes
+
+
+@dataclass(frozen=True)
+class PagedKV8:
+    n_kv: int
+    head_dim: int
+
+    def block_bytes(self, block_size: int, dtype_bytes: int) -> int:
+        # a byte per channel of a key and of a value, two fp32 scales
+        return self.n_kv * (2 * block_size * self.head_dim + 8)
 
 
 @dataclass(frozen=True)
@@ -94,7 +107,14 @@ class SharedCache:
         return 0
 
 
-def default_specs(cfg, n_kv_local: int) -> List[PagedKV]:
+def default_specs(cfg, n_kv_local: int, kv_cache_dtype=None) -> List:
+    if kv_cache_dtype is not None:
+        if kv_cache_dtype != "fp8":
+            raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r}: None or 'fp8'")
+        if cfg.head_dim not in (64, 128) or getattr(cfg, "mrope_section", ()):
+            raise ValueError("an 8-bit cache takes heads of 64 or 128 channels "
+                             "and one position per token")
+        return [PagedKV8(n_kv_local, cfg.head_dim)] * cfg.num_layers
     return [PagedKV(n_kv_local, cfg.head_dim) for _ in range(cfg.num_layers)]
 
 

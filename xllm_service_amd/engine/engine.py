@@ -100,7 +100,12 @@ class LLMEngine:
                  tp_size: int = 1,
                  load_state_path: Optional[str] = None,
                  state_slots: Optional[int] = None,
+                 kv_cache_dtype: Optional[str] = None,
                  seed: int = 0):
+        # kv_cache_dtype: "fp8" keeps keys and values of a dense decoder in 8
+        # bits with a scale for each block and head: half the bytes, so twice the
+        # blocks in the same memory. Preempted sequences recompute, and blocks
+        # move between workers as bytes.
         # model_name: a preset, or a folder holding config.json + safetensors
         self.cfg: ModelConfig = get_config(model_name)
         # tensor parallelism: every rank of the TP group builds its shard;
@@ -140,8 +145,10 @@ class LLMEngine:
         self.model = self.model.eval()
 
         n_kv_local = getattr(self.model, "local_kv_heads", self.cfg.num_kv_heads)
-        specs = ModelRunner.specs_for(self.model, self.cfg)
-        custom_cache = hasattr(self.model, "cache_specs")
+        self.kv_cache_dtype = kv_cache_dtype
+        specs = ModelRunner.specs_for(self.model, self.cfg, kv_cache_dtype)
+        custom_cache = hasattr(self.model, "cache_specs") \
+            or kv_cache_dtype is not None
         from .cache_spec import needs_state_slots
         # recurrent-state layers: one slot per live sequence. Such a state
         # cannot be rebuilt from shared prefix blocks, so prefix reuse is
@@ -199,7 +206,8 @@ class LLMEngine:
                                   enable_graphs=enable_graphs,
                                   max_model_len=max_model_len,
                                   max_graph_batch=min(max_num_seqs, 256),
-                                  num_state_slots=num_state_slots)
+                                  num_state_slots=num_state_slots,
+                                  kv_cache_dtype=kv_cache_dtype)
         if self.cpu_block_manager:
             self.runner.alloc_cpu_caches(self.cpu_block_manager.num_blocks)
         if self.device.type == "cuda":
@@ -623,6 +631,10 @@ class LLMEngine:
         import numpy as np
         idx = torch.tensor(block_ids, dtype=torch.long, device=self.device)
         off = 0
+        need = sum(len(block_ids) * c[0].numel() * c.element_size()
+                   for c in self.runner.paged_tensors())
+        if need != len(data):
+            raise ValueError("the blocks are another cache's")
         for c in self.runner.paged_tensors():
             per = len(block_ids) * c[0].numel() * c.element_size()
             raw = np.frombuffer(data, dtype=np.uint8, count=per, offset=off)

@@ -57,8 +57,15 @@ def _open_tensor(d: dict) -> torch.Tensor:
     return t
 
 
+def _two_tensors(engine):
+    """Caches in 8 bits move as bytes (engine.export_block_bytes)."""
+    if engine.kv_cache_dtype is not None:
+        raise RuntimeError("an 8-bit cache has no shared handles")
+
+
 def export_cache_handles(engine) -> dict:
     """Prefill-side: shareable descriptors for every layer's k/v cache."""
+    _two_tensors(engine)
     handles = []
     for (kc, vc) in engine.runner.kv_caches:
         handles.append([_share_tensor(kc), _share_tensor(vc)])
@@ -84,6 +91,7 @@ class MigrationManager:
                        if engine.device.type == "cuda" else None)
 
     def open_peer(self, name: str, exported: dict):
+        _two_tensors(self.engine)
         self.close_peer(name)
         pc = PeerCache(src_device=int(exported["device"]))
         my_dev = self.engine.device.index or 0

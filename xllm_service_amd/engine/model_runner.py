@@ -14,8 +14,8 @@ import torch
 from xllm_service_amd import ops
 from xllm_service_amd.models.config import ModelConfig
 
-from .cache_spec import (CacheGroup, ConvState, PagedKV, PagedLatent,
-                         RecurrentState, SharedCache, default_specs,
+from .cache_spec import (CacheGroup, ConvState, PagedKV, PagedKV8,
+                         PagedLatent, RecurrentState, SharedCache, default_specs,
                          flat_specs, needs_state_slots)
 from .metadata import AttnMetadata
 from .scheduler import StepPlan
@@ -30,7 +30,8 @@ class ModelRunner:
     def __init__(self, model, cfg: ModelConfig, device: torch.device,
                  num_blocks: int, dtype=torch.bfloat16,
                  enable_graphs: bool = True, max_model_len: int = 4096,
-                 max_graph_batch: int = 256, num_state_slots: int = 0):
+                 max_graph_batch: int = 256, num_state_slots: int = 0,
+                 kv_cache_dtype: Optional[str] = None):
         self.model = model
         self.cfg = cfg
         self.device = device
@@ -39,7 +40,7 @@ class ModelRunner:
         self.graph_runner = None
         self._graph_opts = (enable_graphs and device.type == "cuda",
                             max_model_len, max_graph_batch)
-        self.specs = self.specs_for(model, cfg)
+        self.specs = self.specs_for(model, cfg, kv_cache_dtype)
         self.num_state_slots = num_state_slots
         # one entry per layer, shaped by its spec (engine/cache_spec.py)
         self.kv_caches: List = []
@@ -59,6 +60,9 @@ class ModelRunner:
                 torch.zeros(self.num_blocks, spec.n_kv, BLOCK_SIZE, d,
                             dtype=dtype, device=device)
                 for d in (spec.head_dim, spec.value_dim))
+        if isinstance(spec, PagedKV8):
+            return ops.kv8_cache(self.num_blocks, spec.n_kv, spec.head_dim,
+                                 device)
         if isinstance(spec, PagedLatent):
             return torch.zeros(self.num_blocks, BLOCK_SIZE, spec.width,
                                dtype=dtype, device=device)
@@ -75,12 +79,14 @@ class ModelRunner:
         raise TypeError(f"unknown cache spec {spec!r}")
 
     @staticmethod
-    def specs_for(model, cfg: ModelConfig):
+    def specs_for(model, cfg: ModelConfig, kv_cache_dtype=None):
         if hasattr(model, "cache_specs"):
+            if kv_cache_dtype is not None:
+                raise ValueError("an 8-bit cache is for the dense decoders")
             return list(model.cache_specs())
         n_kv = (model.local_kv_heads if hasattr(model, "local_kv_heads")
                 else cfg.num_kv_heads)
-        return default_specs(cfg, n_kv)
+        return default_specs(cfg, n_kv, kv_cache_dtype)
 
     @property
     def uses_state_slots(self) -> bool:
@@ -93,6 +99,10 @@ class ModelRunner:
         def walk(spec, c):
             if isinstance(spec, PagedKV):
                 out.extend(c[:1] if spec.values_are_keys else c)
+            elif isinstance(spec, PagedKV8):
+                # as bytes: not every operation knows 8-bit floats
+                out.extend((c[0].view(torch.uint8), c[1].view(torch.uint8),
+                            c[2]))
             elif isinstance(spec, PagedLatent):
                 out.append(c)
             elif isinstance(spec, CacheGroup):

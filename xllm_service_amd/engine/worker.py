@@ -766,7 +766,8 @@ class Worker:
                 and self.engine.device.type == "cuda"):
             try:
                 from . import kv_migration
-                if kv_migration.available():
+                if kv_migration.available() and \
+                        self.engine.kv_cache_dtype is None:
                     return "xgmi"
             except Exception:
                 pass
@@ -883,6 +884,8 @@ def main():
                          "per rank with RANK/WORLD_SIZE/MASTER_ADDR set "
                          "(torchrun-style); rank 0 serves RPC, ranks >0 "
                          "run the follower loop")
+    ap.add_argument("--kv-cache-dtype", default=None, choices=["fp8"],
+                    help="keep keys and values of a dense decoder in 8 bits")
     ap.add_argument("--load-state", default=None,
                     help="full (tp=1) state-dict .pt to shard-load")
     args = ap.parse_args()
@@ -897,7 +900,8 @@ def main():
                         seed=args.seed,
                         enable_graphs=not args.no_graphs,
                         max_num_seqs=args.max_num_seqs,
-                        max_batched_tokens=args.max_batched_tokens)
+                        max_batched_tokens=args.max_batched_tokens,
+                        kv_cache_dtype=args.kv_cache_dtype)
         logging.info("TP follower rank %s up", os.environ["RANK"])
         eng.follower_loop()
         return
@@ -915,6 +919,7 @@ def main():
                            enable_graphs=not args.no_graphs,
                            ssd_swap_dir=args.ssd_swap_dir,
                            tp_size=args.tp,
+                           kv_cache_dtype=args.kv_cache_dtype,
                            load_state_path=args.load_state))
 
     async def run():

@@ -76,6 +76,9 @@ class LlamaAttention(nn.Module):
             -1, (self.n_kv_heads, self.head_dim))
         vh = qkv[:, q_sz + kv_sz:].unflatten(
             -1, (self.n_kv_heads, self.head_dim))
+        if len(kv_cache) == 3:                   # 8 bits, with scales
+            return self.o_proj(self._attend_kv8(qh, kh, vh, positions, kv_cache,
+                                                meta, cos_sin))
         k_cache, v_cache = kv_cache
         qh = ops.fused_rope_cache(positions, qh, kh, vh, k_cache, v_cache,
                                   meta.slot_mapping, cos_sin, self.head_dim,
@@ -94,6 +97,22 @@ class LlamaAttention(nn.Module):
                 qh[np_:], k_cache, v_cache, meta.decode_block_tables,
                 meta.decode_seq_lens, self.scale, out=out3[np_:])
         return self.o_proj(out)
+
+    def _attend_kv8(self, qh, kh, vh, positions, cache, meta, cos_sin):
+        qh, kh = ops.rope(positions, qh, kh, cos_sin, self.head_dim,
+                          self.head_dim)
+        ops.reshape_and_cache_kv8(kh, vh, *cache, meta.slot_mapping)
+        np_, nd = meta.num_prefill_tokens, meta.num_decode_tokens
+        out = torch.empty(qh.shape, dtype=qh.dtype, device=qh.device)
+        if np_:
+            ops.paged_attn_prefill_kv8(
+                qh[:np_], *cache, meta.prefill_block_tables, meta.cu_q,
+                meta.prefill_seq_lens, self.scale, out=out[:np_])
+        if nd:
+            ops.paged_attn_decode_kv8(
+                qh[np_:], *cache, meta.decode_block_tables,
+                meta.decode_seq_lens, self.scale, out=out[np_:])
+        return out.flatten(1)
 
 
 class LlamaMLP(nn.Module):

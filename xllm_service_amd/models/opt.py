@@ -30,17 +30,21 @@ class OPTAttention(nn.Module):
         qh = q.contiguous().view(T, self.n_heads, self.head_dim)
         kh = k.contiguous().view(T, self.n_heads, self.head_dim)
         vh = v.contiguous().view(T, self.n_heads, self.head_dim)
-        k_cache, v_cache = kv_cache
-        ops.reshape_and_cache(kh, vh, k_cache, v_cache, meta.slot_mapping)
+        store, prefill, decode = ops.reshape_and_cache, \
+            ops.paged_attn_prefill, ops.paged_attn_decode
+        if len(kv_cache) == 3:                   # 8 bits, with scales
+            store, prefill, decode = ops.reshape_and_cache_kv8, \
+                ops.paged_attn_prefill_kv8, ops.paged_attn_decode_kv8
+        store(kh, vh, *kv_cache, meta.slot_mapping)
         np_, nd = meta.num_prefill_tokens, meta.num_decode_tokens
         out = torch.empty_like(qh)
         if np_:
-            out[:np_] = ops.paged_attn_prefill(
-                qh[:np_], k_cache, v_cache, meta.prefill_block_tables,
+            out[:np_] = prefill(
+                qh[:np_], *kv_cache, meta.prefill_block_tables,
                 meta.cu_q, meta.prefill_seq_lens, self.scale)
         if nd:
-            out[np_:] = ops.paged_attn_decode(
-                qh[np_:], k_cache, v_cache, meta.decode_block_tables,
+            out[np_:] = decode(
+                qh[np_:], *kv_cache, meta.decode_block_tables,
                 meta.decode_seq_lens, self.scale)
         return self.out_proj(out.view(T, -1))
 

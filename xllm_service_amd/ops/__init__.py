@@ -232,7 +232,8 @@ def reshape_and_cache_kv8(k, v, k_cache, v_cache, kv_scale, slot_mapping):
     """New keys and values [tokens, n_kv, head_dim] into their slots (page * 16 +
     offset; -1, or outside of the cache: skipped). Tokens of one page must stand
     side by side in slot_mapping, as those of a sequence do, with none but skipped
-    ones among them; of two for the same slot the later one stays.
+    ones among them (so no two sequences of a call write to one page); of two for the
+    same slot the later one stays.
 
     Where the token at offset 0 of a page is among them the page begins anew: its
     scale is the least power of two whose multiple of 448 holds all of them, and
@@ -240,7 +241,7 @@ def reshape_and_cache_kv8(k, v, k_cache, v_cache, kv_scale, slot_mapping):
     if the scale has to grow they are rounded to it once more (which changes only
     those that become subnormal). What is not finite is held as a NaN and does not
     count for the scale."""
-    if k.is_cuda:
+    if kv_scale.is_cuda:
         _require_ext()
         _ops.reshape_and_cache_kv8(k, v, k_cache, v_cache, kv_scale,
                                    slot_mapping)
@@ -254,7 +255,7 @@ def paged_attn_decode_kv8(q, k_cache, v_cache, kv_scale, block_tables, seq_lens,
     head_dim] bf16, at most 16 heads for each of the cache's. Sequences without
     keys give zeros. Entries of a table that name no page count as page 0, tokens
     behind the end of a table do not count."""
-    if q.is_cuda:
+    if kv_scale.is_cuda:
         _require_ext()
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -271,7 +272,7 @@ def paged_attn_prefill_kv8(q, k_cache, v_cache, kv_scale, block_tables, cu_q,
     head_dim] bf16, those of sequence i from cu_q[i] to cu_q[i + 1]; causal, the
     last of them sees all seq_lens[i] keys. Rows that see no key give zeros, rows
     behind the last sequence stay as they were. Tables as for decoded rows."""
-    if q.is_cuda:
+    if kv_scale.is_cuda:
         _require_ext()
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
