@@ -55,10 +55,12 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
   constexpr int TILE = PF_KT * D;            // elements of a K or V tile
   __shared__ __attribute__((aligned(1024))) unsigned short
       kv_lds[2 * PL_BUFS * TILE];
-  // CACHE8: pages with a value that is a NaN, and which ones are, by channel
-  __shared__ int nan_on[CACHE8 ? PL_BUFS * 4 : 1];
+  // CACHE8, of the tiles that not all rows see all of: pages with a value that is a NaN,
+  // and which ones are, by channel
+  constexpr int EDGES = PL_ROWS / PF_KT + 1;
+  __shared__ int nan_on[CACHE8 ? EDGES * 4 : 1];
   __shared__ __attribute__((aligned(8))) unsigned short
-      nan_at[CACHE8 ? PL_BUFS * D * 4 : 1];
+      nan_at[CACHE8 ? EDGES * D * 4 : 1];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -185,7 +187,9 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
                        : (page4 * PF_BS + (lane & 15)) * D +
                              (((lane >> 4 << 1) ^ mr_swz_rows<D>(lane & 15)) << 3);
   const int more8 = half ? 64 * PF_KT : 64;
-  const int least8 = min(ctx + row0 / G + 1, room);   // fewest keys of a row of all
+  // the first tile that some row of the workgroup does not see all of
+  const int first8 = max(min(ctx + row0 / G + 1, room), 0) / PF_KT;
+  if (CACHE8 && half && lane < EDGES) nan_on[lane * 4 + page4] = 0;
   auto convert8 = [&](unsigned j) {
     if (half) {
       const int t = (int)j - 1;
@@ -194,20 +198,19 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
         page8[0] = kv8_first(page8[0], keys);
         page8[1] = kv8_first(page8[1], keys);
       }
-      // uniform: some row of the workgroup does not see all of the tile
-      if (t * PF_KT + PF_KT > least8) {
+      // uniform: a NaN there would reach rows that do not see it, as 0 times one is one
+      if (t >= first8 && t < n) {
+        const int e = t - first8;
         bool any = false;
 #pragma unroll
         for (int i = 0; i < 2; i++)
           any |= (kv8_nan(page8[i].x) | kv8_nan(page8[i].y) | kv8_nan(page8[i].z) |
                   kv8_nan(page8[i].w)) != 0;
-        any = __any(any);
-        if (lane == 0) nan_on[j % PL_BUFS * 4 + page4] = any;
-        if (any) {
+        if (__any(any)) {
+          if (lane == 0) nan_on[e * 4 + page4] = 1;
 #pragma unroll
           for (int i = 0; i < 2; i++)
-            nan_at[(j % PL_BUFS * D + lane + 64 * i) * 4 + page4] =
-                kv8_drop_nan(page8[i]);
+            nan_at[(e * D + lane + 64 * i) * 4 + page4] = kv8_drop_nan(page8[i]);
         }
       }
     }
@@ -336,27 +339,6 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
     }
   };
 
-  // values of tile t that are NaNs, zeros in its buffer: for the rows that see them
-  auto nans = [&](int t) {
-    if constexpr (CACHE8) {
-      const int buf = (t + 1) % PL_BUFS, k0 = t * PF_KT;
-      if (k0 + PF_KT <= least8) return;          // uniform
-      const int* on = nan_on + buf * 4;
-      if ((on[0] | on[1] | on[2] | on[3]) == 0) return;
-      unsigned long long sees =
-          limit - k0 >= 64 ? ~0ull : (1ull << max(limit - k0, 0)) - 1;
-      for (int w = 0; w < 4; w++)
-        if (!on[w]) sees &= ~(0xffffull << (16 * w));
-      const auto* nan = reinterpret_cast<const unsigned long long*>(nan_at) + buf * D;
-#pragma unroll
-      for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-        for (int r = 0; r < 16; r++)
-          if (nan[dt * 32 + 8 * (r >> 2) + 4 * h + (r & 3)] & sees)
-            o_acc[dt][r] = NAN;
-    }
-  };
-
   // tiles with keys that this wave's rows see
   const unsigned mine =
       wave_on ? (unsigned)(max(wmax, 0) + PF_KT - 1) / PF_KT : 0;
@@ -422,7 +404,6 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
       __builtin_amdgcn_sched_barrier(0);
       fetch_k(fk, kt, 0);
       values(g, 3);
-      nans((int)j - 1);
       __builtin_amdgcn_sched_barrier(0);
       all_scores(fk, kt);
       __builtin_amdgcn_s_setprio(0);
@@ -434,7 +415,6 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
       fetch_v(f, kt + TILE, st);
       values(f, st);
     }
-    nans((int)j - 1);
     __builtin_amdgcn_s_setprio(0);
     if ((int)j < n) meet(2);
     j++;
@@ -449,6 +429,28 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
   if (!half) meet(2);
   // loads past the ends are still on their way to LDS
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if constexpr (CACHE8) {
+    // values that are NaNs, zeros in their tiles: for the rows that see them
+    const int from = first8 * PF_KT;
+    for (int e = 0; e < EDGES; e++) {
+      unsigned long long sees = limit - from >= PF_KT * (e + 1) ? ~0ull
+          : (1ull << min(max(limit - from - PF_KT * e, 0), PF_KT - 1)) - 1;
+      bool any = false;
+      for (int w = 0; w < 4; w++) {
+        const bool on = __builtin_amdgcn_readfirstlane(nan_on[e * 4 + w]);
+        if (!on) sees &= ~(0xffffull << (16 * w));
+        any |= on;
+      }
+      if (!any) continue;
+      const auto* nan = reinterpret_cast<const unsigned long long*>(nan_at) + e * D;
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          if (nan[dt * 32 + 8 * (r >> 2) + 4 * h + (r & 3)] & sees)
+            o_acc[dt][r] = NAN;
+    }
+  }
 
   // ---- epilogue: o_acc[dt][r] = O[row][dt*32 + 8*(r>>2) + 4h + (r&3)] --------
   l = pair_sum(l);

@@ -379,10 +379,12 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
   constexpr int TILE = PF_KT * D;            // elements of a K or V tile
   __shared__ __attribute__((aligned(1024))) unsigned short
       kv_lds[KG * 4 * TILE];
-  // CACHE8: pages with a value that is a NaN, and which ones are, by channel
-  __shared__ int nan_on[CACHE8 ? KG * 8 : 1];
+  // CACHE8, of the tiles that not all rows see all of: pages with a value that is a NaN,
+  // and which ones are, by channel
+  constexpr int EDGES = PF_ROWS / PF_KT + 1;
+  __shared__ int nan_on[CACHE8 ? KG * EDGES * 4 : 1];
   __shared__ __attribute__((aligned(8))) unsigned short
-      nan_at[CACHE8 ? KG * 8 * D : 1];
+      nan_at[CACHE8 ? KG * EDGES * 4 * D : 1];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -547,8 +549,9 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
           reinterpret_cast<const char*>(v_cache) + from + i * 1024);
     }
   };
-  const int least8 =                             // fewest keys of a row of all
-      min(ctx + pf_div(row0, by_G, sG) + 1, room);
+  // the first tile that some row of the workgroup does not see all of
+  const int first8 = max(min(ctx + pf_div(row0, by_G, sG) + 1, room), 0) / PF_KT;
+  if (CACHE8 && lane < EDGES) nan_on[(kg * EDGES + lane) * 4 + wid] = 0;
   // ... and from there to their tile
   auto settle = [&](int t, int buf) {
     unsigned short* dst = kv_lds + (kg * 2 + buf) * 2 * TILE;
@@ -557,21 +560,19 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
 #pragma unroll
       for (int i = 0; i < N8; i++) v8[i] = kv8_first(v8[i], keys);
     }
-    // Uniform: some row of the workgroup does not see all of the tile. A NaN there
-    // would reach it, as 0 times one is one.
-    if (t * PF_KT + PF_KT > least8) {
+    // uniform: a NaN there would reach rows that do not see it, as 0 times one is one
+    if (t >= first8) {
+      const int e = kg * EDGES + t - first8;
       bool any = false;
 #pragma unroll
       for (int i = 0; i < N8; i++)
         any |= (kv8_nan(v8[i].x) | kv8_nan(v8[i].y) | kv8_nan(v8[i].z) |
                 kv8_nan(v8[i].w)) != 0;
-      any = __any(any);
-      if (lane == 0) nan_on[(kg * 2 + buf) * 4 + wid] = any;
-      if (any) {
+      if (__any(any)) {
+        if (lane == 0) nan_on[e * 4 + wid] = 1;
 #pragma unroll
         for (int i = 0; i < N8; i++)
-          nan_at[((kg * 2 + buf) * D + lane + 64 * i) * 4 + wid] =
-              kv8_drop_nan(v8[i]);
+          nan_at[(e * D + lane + 64 * i) * 4 + wid] = kv8_drop_nan(v8[i]);
       }
     }
 #pragma unroll
@@ -719,21 +720,27 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
         for (int e = 0; e < TERMS; e++)
           o_acc[dt] = mr_mma(a, p[e][st], o_acc[dt]);
       }
-    if constexpr (CACHE8) {
-      // values that are NaNs, zeros in the tile: for the rows that see them
-      const int* on = nan_on + (kg * 2 + buf) * 4;
-      if (k0 + PF_KT > least8 && (on[0] | on[1] | on[2] | on[3]) != 0) {
-        u64 sees = limit - k0 >= 64 ? ~0ull : (1ull << max(limit - k0, 0)) - 1;
-        for (int w = 0; w < 4; w++)
-          if (!on[w]) sees &= ~(0xffffull << (16 * w));
-        const u64* nan = reinterpret_cast<const u64*>(nan_at) + (kg * 2 + buf) * D;
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-          for (int r = 0; r < 16; r++)
-            if (nan[dt * 32 + 8 * (r >> 2) + 4 * h + (r & 3)] & sees)
-              o_acc[dt][r] = NAN;
+  }
+  if constexpr (CACHE8) {
+    // values that are NaNs, zeros in their tiles: for the rows that see them
+    const int from = first8 * PF_KT;
+    for (int e = 0; e < EDGES; e++) {
+      unsigned long long sees = limit - from >= PF_KT * (e + 1) ? ~0ull
+          : (1ull << min(max(limit - from - PF_KT * e, 0), PF_KT - 1)) - 1;
+      bool any = false;
+      for (int w = 0; w < 4; w++) {
+        const bool on = __builtin_amdgcn_readfirstlane(nan_on[(kg * EDGES + e) * 4 + w]);
+        if (!on) sees &= ~(0xffffull << (16 * w));
+        any |= on;
       }
+      if (!any) continue;
+      const u64* nan = reinterpret_cast<const u64*>(nan_at) + (kg * EDGES + e) * D;
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          if (nan[dt * 32 + 8 * (r >> 2) + 4 * h + (r & 3)] & sees)
+            o_acc[dt][r] = NAN;
     }
   }
 
