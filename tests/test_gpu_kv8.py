@@ -363,6 +363,47 @@ def test_tables_that_end_before_their_sequence():
     close(got, q, want, table, [0, 4, 9], total, 0.1, 2.0 ** -8)
 
 
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_rows_of_attention_at_any_address(offset):
+    """Queries are read by 16 B, results written by 8: others are copied, and what
+    is around the results stays."""
+    lens, new = [70, 33], [9, 4]
+    cache, want, table = filled(lens, 2, 64, 6)
+    wide = rows(20, 4, 64, 2).to(DEV)
+    q = wide[:13, offset:offset + 256].unflatten(1, (4, 64))
+    big = torch.full((15, 261), 7.0, dtype=torch.bfloat16, device=DEV)
+    out = big[:, offset:offset + 256].unflatten(1, (4, 64))
+    cu = [0, 9, 13]
+    got = ops.paged_attn_prefill_kv8(torch.cat((q, q[:2])), *cache, table.to(DEV),
+                                     ints(cu), ints(lens), 0.1, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    close(out[:13], q, want, table, cu, lens, 0.1, 2.0 ** -8)
+    assert (big[13:] == 7.0).all() and (big[:, :offset] == 7.0).all()
+    assert (big[:, offset + 256:] == 7.0).all()
+    big.fill_(7.0)
+    ops.paged_attn_decode_kv8(q[:2], *cache, table.to(DEV), ints(lens), 0.1,
+                              out=out[:2])
+    close(out[:2], q[:2], want, table, [0, 1, 2], lens, 0.1, 2.0 ** -15)
+    assert (big[2:] == 7.0).all() and (big[:, :offset] == 7.0).all()
+
+
+def test_nothing_to_do():
+    cache, _, table = filled([20], 2, 64, 6)
+    tab, none = table.to(DEV), ints([])
+    q = torch.zeros(0, 4, 64, dtype=torch.bfloat16, device=DEV)
+    assert ops.paged_attn_decode_kv8(q, *cache, tab, ints([20]), 0.1).shape == q.shape
+    assert ops.paged_attn_prefill_kv8(q, *cache, tab, ints([0, 0]), ints([20]),
+                                      0.1).shape == q.shape
+    ops.reshape_and_cache_kv8(q[:, :2], q[:, :2], *cache, ints([], torch.long))
+    slots, pos, cu, used = ops.extend_block_tables(tab[:0], none, none, none, 3)
+    assert slots.tolist() == [-1] * 3 and pos.tolist() == [0] * 3
+    assert cu.tolist() == [0] and used.tolist() == [0]
+    slots, pos, cu, used = ops.extend_block_tables(tab, ints([20]), ints([20]), none,
+                                                   0)
+    assert slots.numel() == pos.numel() == 0
+    assert cu.tolist() == [0, 0] and used.tolist() == [0]
+
+
 def test_negative_scales_and_large_scores():
     lens = [50, 333]
     cache, want, table = filled(lens, 2, 128, 7, big=30.0)

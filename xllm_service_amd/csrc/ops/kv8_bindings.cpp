@@ -126,10 +126,17 @@ int check_attention(const Tensor& out, const Tensor& q, const Cache& c,
   return (int)(q.size(1) / c.n_kv);
 }
 
-void attend_rows(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor kv_scale,
-            Tensor tables, Tensor lens, double scale) {
+// where results go: made here where the caller has none, 1 us less than by torch.empty
+Tensor place_of(const c10::optional<Tensor>& out, const Tensor& q) {
+  return out.has_value() ? *out : at::empty(q.sizes(), q.options());
+}
+
+Tensor attend_rows(Tensor q, Tensor k_cache, Tensor v_cache, Tensor kv_scale,
+                   Tensor tables, Tensor lens, double scale,
+                   c10::optional<Tensor> to) {
   const Cache c = check_cache(k_cache, v_cache, kv_scale);
   const c10::DeviceGuard guard(kv_scale.device());
+  const Tensor out = place_of(to, q);
   const int G = check_attention(out, q, c, kv_scale);
   check_ints(tables, kv_scale, 2, "block_tables");
   check_ints(lens, kv_scale, 1, "seq_lens");
@@ -138,12 +145,11 @@ void attend_rows(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor kv
   TORCH_CHECK(tables.size(0) >= S && lens.size(0) >= S,
               "kv8: a table and a length for each sequence");
   TORCH_CHECK(tables.size(1) < (1L << 26), "kv8: tables too wide");
-  if (S == 0) return;
+  if (S == 0) return out;
   if (!on_bytes(out, 8)) {                  // results are written by 8 B
-    auto rows = torch::empty(q.sizes(), q.options());
-    attend_rows(rows, q, k_cache, v_cache, kv_scale, tables, lens, scale);
-    out.copy_(rows);
-    return;
+    out.copy_(attend_rows(q, k_cache, v_cache, kv_scale, tables, lens, scale,
+                          c10::nullopt));
+    return out;
   }
   if (!on_bytes(q, 16)) q = q.clone(at::MemoryFormat::Contiguous);
   const int width = tables.size(1);
@@ -162,12 +168,15 @@ void attend_rows(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor kv
                           lens.data_ptr<int>(), ws_ml, ws_o, (float)scale, S, H,
                           c.n_kv, c.D, width, c.blocks, q.stride(0), out.stride(0),
                           stream_of(kv_scale));
+  return out;
 }
 
-void attend_prompts(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor kv_scale,
-             Tensor tables, Tensor cu_q, Tensor lens, double scale) {
+Tensor attend_prompts(Tensor q, Tensor k_cache, Tensor v_cache, Tensor kv_scale,
+                      Tensor tables, Tensor cu_q, Tensor lens, double scale,
+                      c10::optional<Tensor> to) {
   const Cache c = check_cache(k_cache, v_cache, kv_scale);
   const c10::DeviceGuard guard(kv_scale.device());
+  const Tensor out = place_of(to, q);
   const int G = check_attention(out, q, c, kv_scale);
   check_ints(tables, kv_scale, 2, "block_tables");
   check_ints(cu_q, kv_scale, 1, "cu_q");
@@ -178,12 +187,11 @@ void attend_prompts(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor
               "kv8: a table and a length for each sequence");
   TORCH_CHECK(tables.size(1) < (1L << 26), "kv8: tables too wide");
   const long T = q.size(0);
-  if (T == 0 || S == 0) return;
-  if (!on_bytes(out, 8)) {
-    auto rows = out.clone(at::MemoryFormat::Contiguous);
-    attend_prompts(rows, q, k_cache, v_cache, kv_scale, tables, cu_q, lens, scale);
-    out.copy_(rows);
-    return;
+  if (T == 0 || S == 0) return out;
+  if (!on_bytes(out, 8)) {                  // rows of no prompt stay as they are
+    out.copy_(attend_prompts(q, k_cache, v_cache, kv_scale, tables, cu_q, lens, scale,
+                             out.clone(at::MemoryFormat::Contiguous)));
+    return out;
   }
   if (!on_bytes(q, 16)) q = q.clone(at::MemoryFormat::Contiguous);
   const long need = xllm::kv8_prefill_scratch(T, S, G, c.n_kv, c.D, width);
@@ -196,6 +204,7 @@ void attend_prompts(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor
                            (float)scale, (int)q.size(1), c.n_kv, c.D, width,
                            c.blocks, q.stride(0), out.stride(0),
                            stream_of(kv_scale));
+  return out;
 }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> plan_tables(Tensor tables, Tensor seq_lens,

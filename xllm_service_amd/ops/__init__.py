@@ -257,11 +257,8 @@ def paged_attn_decode_kv8(q, k_cache, v_cache, kv_scale, block_tables, seq_lens,
     behind the end of a table do not count."""
     if kv_scale.is_cuda:
         _require_ext()
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _ops.paged_attn_decode_kv8(out, q, k_cache, v_cache, kv_scale,
-                                   block_tables, seq_lens, scale)
-        return out
+        return _ops.paged_attn_decode_kv8(q, k_cache, v_cache, kv_scale,
+                                          block_tables, seq_lens, scale, out)
     return ref.paged_attn_decode_kv8(q, k_cache, v_cache, kv_scale, block_tables,
                                      seq_lens, scale, out)
 
@@ -274,11 +271,9 @@ def paged_attn_prefill_kv8(q, k_cache, v_cache, kv_scale, block_tables, cu_q,
     behind the last sequence stay as they were. Tables as for decoded rows."""
     if kv_scale.is_cuda:
         _require_ext()
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _ops.paged_attn_prefill_kv8(out, q, k_cache, v_cache, kv_scale,
-                                    block_tables, cu_q, seq_lens, scale)
-        return out
+        return _ops.paged_attn_prefill_kv8(q, k_cache, v_cache, kv_scale,
+                                           block_tables, cu_q, seq_lens, scale,
+                                           out)
     return ref.paged_attn_prefill_kv8(q, k_cache, v_cache, kv_scale,
                                       block_tables, cu_q, seq_lens, scale, out)
 
