@@ -374,7 +374,6 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void kv8_decode16_kernel(
   const int k_page = c16 >> 2;               // of the tile, that this lane has keys of
   const unsigned k_off = quad * 256 + (c16 & 3) * 16, v_off = c16 * 16;
   uint4 kr[4][NC], vr[DT];
-  float ks = 0.0f, vs = 0.0f;
   auto load_k = [&](int n) {
     const int at = 4 * (n - tb) + k_page;
     const uint4* from = reinterpret_cast<const uint4*>(
@@ -383,7 +382,6 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void kv8_decode16_kernel(
     for (int t = 0; t < 4; t++)
 #pragma unroll
       for (int i = 0; i < NC; i++) kr[t][i] = from[i * 64 + t * 4];
-    ks = __shfl(sizes.x, at, 64);
   };
   auto load_v = [&](int n) {
     const int at = 4 * (n - tb) + quad;
@@ -391,7 +389,6 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void kv8_decode16_kernel(
         v_cache + ((long)__shfl(ids, at, 64) * n_kv + kvh) * PAGE + v_off);
 #pragma unroll
     for (int i = 0; i < DT; i++) vr[i] = from[i * 16];
-    vs = __shfl(sizes.y, at, 64);
   };
   if (SPLIT && parts > 1 && tid == 0) paged_open(meet.count + unit, seen, meet.tag);
   if (i0 < n_tiles) {
@@ -400,6 +397,9 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void kv8_decode16_kernel(
   }
   for (int t = i0, n = 0; t < n_tiles; t += step, n++) {
     const bool more = t + step < n_tiles;
+    // (asked for no earlier: the first values would wait for the scales)
+    const float ks = __shfl(sizes.x, 4 * (n - tb) + k_page, 64);
+    float vs = __shfl(sizes.y, 4 * (n - tb) + quad, 64);
     f4 s[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
