@@ -344,14 +344,16 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void kv8_decode16_kernel(
   const int* btab = block_tables + (long)seq * max_blocks;
   int tb = 0, ids = 0;
   float2 sizes = {0.0f, 0.0f};
-  auto look_up = [&](int n) {
-    if (max_blocks <= 0) return;
-    const int id = btab[min(4 * (i0 + (n + (lane >> 2)) * step) + (lane & 3),
-                            max_blocks - 1)];
+  auto entry = [&](int n) {
+    return max_blocks <= 0
+        ? 0
+        : btab[min(4 * (i0 + (n + (lane >> 2)) * step) + (lane & 3), max_blocks - 1)];
+  };
+  auto look_up = [&](int id) {
     ids = (unsigned)id < (unsigned)n_blocks ? id : 0;
     sizes = kv_scale[(long)ids * n_kv + kvh];
   };
-  look_up(0);
+  const int id0 = entry(0);
 
   const int col = c16 & 7;
   const bool second = c16 >= 8;              // second terms of column col
@@ -366,6 +368,8 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void kv8_decode16_kernel(
                 q + (long)seq * q_stride + (long)head * D +
                 16 * (4 * (i >> 1) + quad) + 8 * (i & 1)) ^
             sc.flip;
+  __builtin_amdgcn_sched_barrier(0);         // queries are asked for before the wait
+  look_up(id0);
   f4 o_acc[DT];
 #pragma unroll
   for (int i = 0; i < DT; i++) o_acc[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -414,7 +418,7 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void kv8_decode16_kernel(
     if (more) {
       if (n + 1 - tb == 16) {                // this tile's values are on their way
         tb += 16;
-        look_up(tb);
+        look_up(entry(tb));
       }
       load_k(n + 1);
     }
