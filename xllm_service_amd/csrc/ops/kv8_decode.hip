@@ -11,8 +11,9 @@
 // long sequences are split over workgroups, the last of which merges (paged_merge.h).
 //
 // Bound by memory where there is much of it: 128 sequences of 1-2 k keys, 32/8 heads of
-// 128, 79 us, 5.1 TB/s (a large copy: 4.97; four times the sequences 5.5 TB/s; bf16 pages
-// 142 us); 6 of 9-20 k, 28/4 heads, 22 us. One of 776 7.0: a launch, a chain of table,
+// 128, 76 to 82 us by card, 5.3 to 4.9 TB/s (a large copy: 5.0; bf16 pages 144 us); 6 of
+// 9-20 k, 28/4 heads, whose 92 MB are longer than the cache before memory 23 (40), and 18.8
+// where they are partly in it. One of 776 6.7 to 7.1 (8.1): a launch, a chain of table,
 // scales and keys, then of four tiles a wave.
 #include "kv8.h"
 #include "paged_stream.h"
@@ -278,9 +279,10 @@ __global__ __launch_bounds__(256, 2) void kv8_decode_kernel(
 // G <= 8 on 16x16x32 products, which have half the columns: half the scores to a lane, 112
 // registers for sums, queries and a tile's keys and values where the other kernel has 160,
 // and so three waves to a SIMD, four for 64-wide heads. Us, that kernel | this one: 6 x
-// 9-20 k of 28/4 heads 26.5 | 24.5, 16 x 0.5-4 k of 32/8 20.2 | 17.6, 24 x 0.6-1.4 k 14.7 | 12.7,
-// 1 x 300 6.2 | 5.4, 128 x 300 23.4 | 21.6, 128 x 1-2 k 82.6 | 84.3 (1024 workgroups are two
-// full turns of it and one and a third of these), 48 of 12 heads of 64 22.7 | 20.7. A tile is 64 keys, four pages, and quarter q of the lanes (l >> 4) has page q:
+// 9-20 k of 28/4 heads 26.5 | 23.0, 16 x 0.5-4 k of 32/8 20.2 | 17.6, 24 x 0.6-1.4 k 14.7 | 12.7,
+// 1 x 300 6.2 | 5.4, 128 x 300 23.4 | 20.8, 128 x 1-2 k 82.6 | 81.7 (1024 workgroups are two
+// full turns of it and one and a third of these), 48 of 12 heads of 64 22.7 | 20.6. A tile
+// is 64 keys, four pages, and quarter q of the lanes (l >> 4) has page q:
 //
 //   keys     row m of set t is token 4 t + (m & 3) of page m >> 2; after four sets a lane
 //            holds the 16 scores of its page, in order
@@ -496,6 +498,8 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void kv8_decode16_kernel(
 // Parts as over bf16 pages, by tiles of 64 keys where G <= 8. Few pairs are split later,
 // from 14 tiles on: a wave's second and third tile cost less than the merge. Us, whole |
 // in parts: 1 x 776 keys 7.0 | 7.3, 8 x 500 6.4 | 7.8, 1 x 2000 10.5 | 7.6, 8 x 2000 13.3 | 11.0.
+// Up to 512 or 768 workgroups, with parts of 2 to 8 tiles, in place of 256 took as long or
+// longer: 6 x 9-20 k 23.0 | 23.9 to 25.8, 4 x 8-30 k 34.7 | 36 to 37, 1 x 20 k 14.2 | 14.3 to 22.9.
 // Many pairs gain nothing by parts here either: 128 sequences of 1-2 k keys 84 in one, 86
 // in two, 88 in four; 48 of 12 heads of 64, up to 2000 keys, 20.8, 22.6, 22.4.
 static PagedSplit kv8_split(long num_seqs, int n_kv, int G, long max_blocks) {

@@ -1,5 +1,5 @@
 // Paged attention of prompt rows over a cache held in 8 bits (kv8.h), bf16 in and out,
-// causal: the kernels of paged_rows.h over such pages.
+// causal: few rows by kv8_short.h, long prompts by paged_long.h, the rest by paged_rows.h.
 //
 // Weights are rounded to bf16, as over bf16 pages of 128-wide heads: 2^-8 of each at
 // most, a thirty-second of what the values themselves were rounded by.

@@ -33,7 +33,8 @@ namespace xllm {
 
 // CACHE8: pages of 8 bits (kv8.h), as in paged_rows.h: among its products a wave converts
 // its page of two steps later, as values are read from the half step before their bundle
-// on, and asks for the one after it.
+// on, and asks for the one after it: 7.9 k tokens over up to 3.1 k, 32/8 heads, 296 us, over bf16
+// pages 285 (both by the power that the products draw).
 template <bool CACHE8>
 __global__ __launch_bounds__(512) void paged_attn_long_kernel(
     unsigned short* __restrict__ out,        // [total_q, n_qheads, D]
