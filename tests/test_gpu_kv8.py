@@ -149,6 +149,25 @@ def test_tables_from_lengths(seqs, most_old, most_new, short):
         assert torch.equal(a.cpu(), b)
 
 
+# sums of what is no length of a sequence would pass 32 bits
+@pytest.mark.parametrize("seqs", [3, 256, 600, 1500])
+@pytest.mark.parametrize("room", [0, 100])
+def test_tables_from_lengths_of_any_size(seqs, room):
+    most = 2 ** 31 - 1
+    old = torch.zeros(seqs, dtype=torch.int32)
+    new = torch.full_like(old, most)
+    old[seqs // 2:], new[-1] = most, -most - 1
+    old[:1], new[:1] = 3, 40
+    free = torch.arange(7, dtype=torch.int32) * 3
+    table = torch.arange(seqs * 3, dtype=torch.int32).reshape(seqs, 3)
+    there = table.to(DEV)
+    got = ops.extend_block_tables(there, old.to(DEV), new.to(DEV), free.to(DEV), room)
+    want = ops.extend_block_tables(table, old, new, free, room)
+    assert torch.equal(there.cpu(), table)
+    for a, b in zip(got, want):
+        assert torch.equal(a.cpu(), b)
+
+
 # ---- attention ---------------------------------------------------------------
 SHAPES = [(2, 4, 128), (1, 7, 128), (3, 1, 64), (2, 16, 128), (2, 12, 64),
           (1, 1, 128)]
@@ -618,6 +637,7 @@ def test_refusals():
     no(e, tab[:2], lens, lens, lens, 4)
     no(e, tab, lens.cpu(), lens, lens, 4)
     no(e, tab, lens, lens, lens, -1)
+    no(e, tab, lens, lens, lens, 2 ** 20 + 1)
     no(e, tab.expand(4, 3), lens, lens, lens, 4)
 
 

@@ -123,6 +123,22 @@ def test_tables_from_lengths(old, new, free, width, room):
                                       torch.int32]
 
 
+def test_tables_from_lengths_of_any_size():
+    most = 2 ** 31 - 1
+    old = torch.tensor([3, 0, most, most]).int()
+    new = torch.tensor([40, most, most, -most]).int()
+    table = torch.zeros(4, 3, dtype=torch.int32)
+    slots, pos, cu, used = ops.extend_block_tables(
+        table, old, new, torch.arange(1, 8).int(), 100)
+    # lengths count as 2^24 - 1 at most, which is 2^20 pages
+    assert table.tolist() == [[0, 1, 2], [3, 4, 5], [0, 0, 0], [0, 0, 0]]
+    assert pos.tolist() == [*range(3, 40), *range(63)]
+    assert cu.tolist() == [0, 37, 100, 100, 100]
+    assert used.tolist() == [2 + 2 ** 20]
+    with pytest.raises(RuntimeError):
+        ops.extend_block_tables(table, old, new, table[0], 2 ** 20 + 1)
+
+
 def test_a_run_of_them():
     """Three steps of two sequences: planned, written and attended, against the
     same over all tokens at once."""

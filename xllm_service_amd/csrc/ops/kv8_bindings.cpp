@@ -221,7 +221,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> plan_tables(Tensor tables, Tensor seq
   const long S = seq_lens.size(0);
   TORCH_CHECK(new_lens.size(0) == S && tables.size(0) >= S,
               "a new length and a table for each sequence");
-  TORCH_CHECK(n_tokens >= 0 && n_tokens < (1L << 30) && S < (1L << 24) &&
+  TORCH_CHECK(n_tokens >= 0 && n_tokens <= (1L << 20) && S < (1L << 24) &&
                   tables.size(1) < (1L << 26) && free_blocks.size(0) < (1L << 30),
               "too many tokens, sequences or pages");
   // one piece of memory for all four: an allocation takes 1.2 us

@@ -16,7 +16,11 @@ namespace xllm {
 // Us in a captured graph, where a launch takes 3.2: one sequence 3.3, 128 that grow by a
 // token 4.1, 600 by 36 k tokens 5.8, 1000 by 39 k 6.0. A call from the host takes 5.5,
 // with the memory of its results.
+//   Sums of 32 bits hold whatever lengths a caller has: those past KV8_LONGEST, 2^20 pages,
+// count as that, no sequence counts for more tokens than there is room for (2^20 at most,
+// kv8_bindings.cpp), and sums of rounds stop at that room and at 2^30 - 1 pages.
 // SEQS: sequences of a round, threads.
+constexpr int KV8_LONGEST = (1 << 24) - 1;
 template <int SEQS>
 __global__ __launch_bounds__(SEQS) void kv8_plan_kernel(
     int* __restrict__ tables, const int* __restrict__ seq_lens,
@@ -32,10 +36,10 @@ __global__ __launch_bounds__(SEQS) void kv8_plan_kernel(
   int tokens = 0, pages = 0;               // of the rounds before
   for (int base = 0; base < n_seqs; base += SEQS) {
     const int i = base + tid;
-    const int old = i < n_seqs ? max(seq_lens[i], 0) : 0;
-    const int now = i < n_seqs ? max(new_lens[i], old) : 0;
+    const int old = i < n_seqs ? min(max(seq_lens[i], 0), KV8_LONGEST) : 0;
+    const int now = i < n_seqs ? min(max(new_lens[i], old), KV8_LONGEST) : 0;
     const int first = old / KV8_PAGE + (old % KV8_PAGE != 0);
-    const int mine_t = now - old;
+    const int mine_t = min(now - old, n_tokens);
     int t = pf_scan<true>(mine_t);
     int p = pf_scan<true>(now / KV8_PAGE + (now % KV8_PAGE != 0) - first);
     if (lane == 63) sums[0][wid] = t, sums[1][wid] = p;
@@ -84,12 +88,12 @@ __global__ __launch_bounds__(SEQS) void kv8_plan_kernel(
       if ((unsigned)col < (unsigned)width)
         tables[(base + s) * table_stride + col] = free_blocks[x];
     }
-    tokens = tok_at[SEQS];
-    pages = page_at[SEQS];
+    tokens = min(tok_at[SEQS], n_tokens);
+    pages = min(page_at[SEQS], (1 << 30) - 1);
     __syncthreads();
   }
   if (me == 0 && tid == 0) {
-    cu_q[n_seqs] = min(tokens, n_tokens);
+    cu_q[n_seqs] = tokens;
     *used = pages;
   }
   // rows behind the last token

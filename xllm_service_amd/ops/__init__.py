@@ -216,7 +216,8 @@ def extend_block_tables(block_tables, seq_lens, new_lens, free_blocks,
     (sequence, position), slot_mapping and positions (int64 [num_tokens]), cu_q
     (int32 [sequences + 1]) and the pages taken (int32 [1]).
 
-    num_tokens: room for new tokens, at least their sum. Rows behind the last one
+    num_tokens: room for new tokens, at least their sum, at most 2^20. Lengths past
+    2^24 - 1 count as that. Rows behind the last one
     have slot -1 and position 0. Pages that free_blocks or a table's columns have no
     place for are not written and their tokens have slot -1: the step fits if the
     pages taken are no more than free_blocks has and lengths no more than tables."""

@@ -167,13 +167,16 @@ KV8_PAGE = 16
 def extend_block_tables(block_tables, seq_lens, new_lens, free_blocks,
                         num_tokens):
     W, F = block_tables.shape[1], free_blocks.shape[0]
+    if not 0 <= num_tokens <= 1 << 20:
+        raise RuntimeError("too many tokens, sequences or pages")
+    longest = (1 << 24) - 1
     slots = torch.full((num_tokens,), -1, dtype=torch.long)
     positions = torch.zeros(num_tokens, dtype=torch.long)
     cu_q = [0]
     at = pages = 0
     for i, (old, new) in enumerate(zip(seq_lens.tolist(), new_lens.tolist())):
-        old = max(old, 0)
-        new = max(new, old)
+        old = min(max(old, 0), longest)
+        new = min(max(new, old), longest)
         held, need = -(-old // KV8_PAGE), -(-new // KV8_PAGE)
         for col in range(held, min(need, W)):
             if pages + col - held < F:
@@ -188,6 +191,7 @@ def extend_block_tables(block_tables, seq_lens, new_lens, free_blocks,
         at = min(at + new - old, num_tokens)
         pages += need - held
         cu_q.append(at)
+    pages = min(pages, (1 << 30) - 1)
     return (slots, positions, torch.tensor(cu_q, dtype=torch.int32),
             torch.tensor([pages], dtype=torch.int32))
 
