@@ -260,6 +260,23 @@ def test_engine_first_logits():
     assert 0 < diff < bound
 
 
+@pytest.mark.parametrize("heads,kv_heads,good", [
+    (32, 2, True), (34, 2, False), (17, 1, False)])
+def test_query_heads_per_key_head(heads, kv_heads, good):
+    import dataclasses
+
+    from xllm_service_amd.engine.cache_spec import PagedKV8, default_specs
+    from xllm_service_amd.models.config import get_config
+    cfg = dataclasses.replace(get_config("llama-tiny"), num_heads=heads,
+                              num_kv_heads=kv_heads)
+    if good:
+        assert isinstance(default_specs(cfg, kv_heads, "fp8")[0], PagedKV8)
+    else:
+        with pytest.raises(ValueError, match="16 query heads"):
+            default_specs(cfg, kv_heads, "fp8")
+    assert len(default_specs(cfg, kv_heads)) == cfg.num_layers
+
+
 def test_engine_holds_twice_the_blocks_and_refuses():
     from xllm_service_amd.engine.cache_spec import default_specs
     from xllm_service_amd.models.config import get_config

@@ -114,6 +114,9 @@ def default_specs(cfg, n_kv_local: int, kv_cache_dtype=None) -> List:
         if cfg.head_dim not in (64, 128) or getattr(cfg, "mrope_section", ()):
             raise ValueError("an 8-bit cache takes heads of 64 or 128 channels "
                              "and one position per token")
+        if cfg.num_heads > 16 * cfg.num_kv_heads:
+            raise ValueError("an 8-bit cache takes 16 query heads per key head "
+                             "at most")
         return [PagedKV8(n_kv_local, cfg.head_dim)] * cfg.num_layers
     return [PagedKV(n_kv_local, cfg.head_dim) for _ in range(cfg.num_layers)]
 

@@ -146,6 +146,9 @@ class LLMEngine:
 
         n_kv_local = getattr(self.model, "local_kv_heads", self.cfg.num_kv_heads)
         self.kv_cache_dtype = kv_cache_dtype
+        if kv_cache_dtype is not None and self.device.type == "cuda" \
+                and dtype != torch.bfloat16:
+            raise ValueError("an 8-bit cache takes bf16 models on a GPU")
         specs = ModelRunner.specs_for(self.model, self.cfg, kv_cache_dtype)
         custom_cache = hasattr(self.model, "cache_specs") \
             or kv_cache_dtype is not None
