@@ -631,6 +631,11 @@ def test_refusals():
     no(p, x, k8, v8, s, tab, cu[:0], lens, 1.0)
     no(p, x, k8, v8, s, tab[:0], cu, lens, 1.0)
     no(p, x, k8, v8, s[:2], tab, cu, lens, 1.0)
+    many = ints([0]).expand(2 ** 21 + 1).contiguous()   # of two heads each
+    with pytest.raises(RuntimeError, match="too many sequences"):
+        d(x[:1].expand(2 ** 21, 2, 64), k8, v8, s, many[:, None], many, 1.0)
+    with pytest.raises(RuntimeError, match="too many sequences"):
+        p(x, k8, v8, s, many[:, None], many, many, 1.0)
     e = ops.extend_block_tables
     no(e, tab.long(), lens, lens, lens, 4)
     no(e, tab, lens, lens[:2], lens, 4)

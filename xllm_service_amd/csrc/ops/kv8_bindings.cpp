@@ -126,6 +126,11 @@ int check_attention(const Tensor& out, const Tensor& q, const Cache& c,
   return (int)(q.size(1) / c.n_kv);
 }
 
+// a launch has fewer than 2^32 threads
+void check_grid(long n_seqs, const Cache& c) {
+  TORCH_CHECK(n_seqs * c.n_kv < (1L << 22), "kv8: too many sequences");
+}
+
 // where results go: made here where the caller has none, 1 us less than by torch.empty
 Tensor place_of(const c10::optional<Tensor>& out, const Tensor& q) {
   return out.has_value() ? *out : at::empty(q.sizes(), q.options());
@@ -142,6 +147,7 @@ Tensor attend_rows(Tensor q, Tensor k_cache, Tensor v_cache, Tensor kv_scale,
   check_ints(lens, kv_scale, 1, "seq_lens");
   const int S = q.size(0), H = q.size(1);
   TORCH_CHECK(G <= 16, "kv8: at most 16 query heads for each of the cache's");
+  check_grid(S, c);
   TORCH_CHECK(tables.size(0) >= S && lens.size(0) >= S,
               "kv8: a table and a length for each sequence");
   TORCH_CHECK(tables.size(1) < (1L << 26), "kv8: tables too wide");
@@ -182,6 +188,7 @@ Tensor attend_prompts(Tensor q, Tensor k_cache, Tensor v_cache, Tensor kv_scale,
   check_ints(cu_q, kv_scale, 1, "cu_q");
   check_ints(lens, kv_scale, 1, "seq_lens");
   TORCH_CHECK(cu_q.size(0) > 0, "kv8: cu_q must have an entry more than sequences");
+  check_grid(cu_q.size(0) - 1, c);
   const int S = cu_q.size(0) - 1, width = tables.size(1);
   TORCH_CHECK(tables.size(0) >= S && lens.size(0) >= S,
               "kv8: a table and a length for each sequence");
