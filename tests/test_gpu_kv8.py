@@ -6,7 +6,9 @@ is exact, and one rounding to e4m3 is left. Attention: results are bf16, off by 
 2^-24 D of the sum of their sizes, and what the exponent is made of by 2^-22 more: a
 weight is off by as much of itself, numerator and denominator. Weights of decoded rows
 have two truncated bf16 terms, off by 2^-15 of themselves; those of prompts are
-rounded to bf16, 2^-8."""
+rounded to bf16, by e = 2^-8 / (1 + 2^-8) of themselves at most, and divided by the sum P of
+the rounded ones: a result o is off by |sum (p' - p) (v - o)| / P, and with P at least
+(1 - e) sum p = sum p / (1 + 2^-8) that is 2^-8 (sum p |v| / sum p + |o|) at most."""
 import math
 
 import pytest
@@ -63,7 +65,7 @@ def close(got, q, want, table, cu, total, scale, weights):
     k, v = want.values(0), want.values(1)
     ref, big, most = attend(q, k, v, table, cu, total, scale)
     off = 2.0 ** -24 * q.shape[2] * most + 2.0 ** -22 * most.clamp(min=1.0)
-    bound = 2.0 ** -8 * ref.abs() + (weights + 2 * off) * big + 1e-30
+    bound = (2.0 ** -8 + weights) * ref.abs() + (weights + 2 * off) * big + 1e-30
     diff = (got.cpu().double() - ref).abs()
     assert not diff.isnan().any()
     assert (diff <= bound).all(), float((diff / bound).max())

@@ -54,6 +54,12 @@ XLLM_DEV bf16x8 kv8_wide(unsigned lo, unsigned hi, float scale) {
   __builtin_memcpy(&y, x, 16);
   return y;
 }
+// l and both of a pair of bf16 weights
+XLLM_DEV float kv8_add(unsigned u, float l) {
+  typedef __attribute__((ext_vector_type(2))) __bf16 pair;
+  return __builtin_amdgcn_fdot2_f32_bf16(
+      __builtin_bit_cast(pair, u), __builtin_bit_cast(pair, 0x3f803f80u), l, false);
+}
 // the top bits of those of four e4m3 values that are NaNs (0x7f but for the sign)
 XLLM_DEV unsigned kv8_nan(unsigned u) {
   return ~((~u & 0x7f7f7f7fu) + 0x7f7f7f7fu) & 0x80808080u;

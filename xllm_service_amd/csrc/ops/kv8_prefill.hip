@@ -2,7 +2,9 @@
 // causal: few rows by kv8_short.h, long prompts by paged_long.h, the rest by paged_rows.h.
 //
 // Weights are rounded to bf16, as over bf16 pages of 128-wide heads: 2^-8 of each at
-// most, a thirty-second of what the values themselves were rounded by.
+// most, a sixteenth of what the values themselves were rounded by. What they are
+// divided by is the sum of the rounded ones: made by products of pairs with ones, in half
+// the additions, and exact results where one weight is all there is.
 #include "kv8_short.h"
 #include "paged_long.h"
 

@@ -259,8 +259,9 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
     for (int r = 8 * (st & 1); r < 8 * (st & 1) + 8; r += 2) {
       const float a = __builtin_amdgcn_exp2f(fmaf(s[i][r], c, -mc));
       const float b = __builtin_amdgcn_exp2f(fmaf(s[i][r + 1], c, -mc));
-      l += a + b;
-      reinterpret_cast<unsigned*>(&p[st])[(r & 7) >> 1] = pack_bf16(a, b);
+      const unsigned u = pack_bf16(a, b);
+      l = CACHE8 ? kv8_add(u, l) : l + (a + b);
+      reinterpret_cast<unsigned*>(&p[st])[(r & 7) >> 1] = u;
     }
   };
   // operands of four products: 16 values' rows, or two steps of the keys'

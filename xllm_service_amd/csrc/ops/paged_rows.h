@@ -677,7 +677,11 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
     // same whatever they are scaled by, so there sums are scaled only where one has grown
     // by more than 2^8: 2 of 1.5-2.6 k in a window of 1024 53.4 -> 51.4 us, 911 and 1317
     // capped 64.5 -> 61.8, errors 1-2% smaller. (One rounded to bf16 is exact where it is 1.)
-    if (TERMS > 1 ? __any((mt - m) * c > 8.0f) : __any(mt > m)) {
+    // So too over pages of 8 bits, where sums are of the weights as rounded, so that a row's
+    // only large one counts for what it is: 16 x 60-140 behind 0.3-0.7 k 35.1 -> 32.9, 2000 of 28/4
+    // 49.9 -> 47.4; what results are off by is 0.0021 for 0.0018, of 0.0016 by their own
+    // rounding, where the values' rounding gives 0.02.
+    if (TERMS > 1 || CACHE8 ? __any((mt - m) * c > 8.0f) : __any(mt > m)) {
       const float m_new = fmaxf(m, mt);
       const float alpha =
           __builtin_amdgcn_exp2f((m - (m_new == -INFINITY ? 0.f : m_new)) * c);
@@ -696,10 +700,11 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
       for (int r = 0; r < 16; r += 2) {
         float a = __builtin_amdgcn_exp2f(fmaf(s[i][r], c, -mc));
         float b = __builtin_amdgcn_exp2f(fmaf(s[i][r + 1], c, -mc));
-        l += a + b;
+        if constexpr (!CACHE8) l += a + b;
 #pragma unroll
         for (int e = 0; e < TERMS; e++) {
           const unsigned u = pack_bf16(a, b);
+          if constexpr (CACHE8) l = kv8_add(u, l);
           reinterpret_cast<unsigned*>(
               &p[e][i * 2 + (r >> 3)])[(r & 7) >> 1] = u;
           drop_bf16(a, b, u);
