@@ -6,6 +6,10 @@
 // that go from memory to registers, as for decoded rows (kv8_decode.hip, whose order of
 // keys, values and channels this is): nothing passes through LDS, a CU holds two
 // workgroups, and pulls half as much for a key.
+//
+// Scores by e4m3 products (queries as the sum of two e4m3 terms, pages' scales in the
+// instruction) need no conversion of keys and took 2% less of long chains, but 0.8 us to
+// split the queries: 300 tokens of 32/8 heads 9.1 for 8.2.
 #pragma once
 #include "paged_rows.h"
 
