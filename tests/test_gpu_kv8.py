@@ -339,6 +339,46 @@ def test_prefill_and_odd_lengths(total, heads, per, dim, width):
     close(got, q, want, table, [0, T], [total], 0.09, 2.0 ** -8)
 
 
+
+FAR, LOW = 2 ** 31 - 1, -2 ** 31
+
+
+# a sequence's length need not be what its table holds: row tiles sorted and as they
+# are, keys split over workgroups of one and of several sequences, whole turns, few rows
+@pytest.mark.parametrize("heads,per,dim,new,lens,width", [
+    (16, 4, 128, [80] * 9, [FAR, -9, 80, 2 ** 30, 128, LOW, 3 * 10 ** 8, 100, 0], 8),
+    (24, 1, 128, [300] * 4, [FAR, -9, 300, 200], 19),
+    (16, 1, 64, [300] * 9, [LOW, FAR, 304, 2 ** 30, -1, 5, 300, 0, FAR - 1], 19),
+    (2, 4, 128, [40, 3], [FAR, 2 ** 30], 400),
+    (1, 8, 128, [16] * 15 + [1600], [40000] * 15 + [2 ** 30], 700),
+    (1, 8, 128, [16] * 15 + [1600], [FAR, LOW, 300] * 5 + [FAR], 700),
+    (2, 4, 128, [9], [FAR], 300), (2, 4, 128, [9], [LOW], 300),
+    (24, 8, 128, [600], [FAR], 140), (24, 8, 128, [600], [LOW], 140),
+    (21, 8, 128, [300, 400], [FAR, -9], 140),
+    (21, 8, 128, [300, 400], [LOW, 3 * 10 ** 8], 140),
+    (2, 4, 128, [100], [FAR], 12), (2, 4, 128, [100, 7], [LOW, FAR], 12)])
+def test_prefill_and_lengths_of_any_size(heads, per, dim, new, lens, width):
+    cache, want, table = filled([192] * len(new), heads, dim, 3)
+    table = table.repeat(1, -(-width // 12))[:, :width].contiguous()
+    T = sum(new)
+    q = part(rows(T + 3, heads * per, dim, 6), heads * per, dim)
+    cu = [sum(new[:i]) for i in range(len(new) + 1)]
+    out = torch.full((T + 3, heads * per, dim), 7.0, dtype=torch.bfloat16,
+                     device=DEV)
+    ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints(cu), ints(lens), 0.09,
+                               out=out)
+    close(out[:T], q[:T], want, table, cu, lens, 0.09, 2.0 ** -8)
+    assert (out[T:] == 7.0).all()
+
+
+@pytest.mark.parametrize("heads,per,dim", [(2, 4, 128), (1, 12, 64)])
+def test_decode_and_lengths_of_any_size(heads, per, dim):
+    lens = [FAR, LOW, -1, 2 ** 30, 33]
+    cache, want, table = filled([192] * 5, heads, dim, 3)
+    q = part(rows(5, heads * per, dim, 6), heads * per, dim)
+    got = ops.paged_attn_decode_kv8(q, *cache, table.to(DEV), ints(lens), 0.09)
+    close(got, q, want, table, list(range(6)), lens, 0.09, 2.0 ** -15)
+
 def test_rows_without_keys():
     """Lengths of zero and below, chunks longer than their sequence, tables without
     columns."""

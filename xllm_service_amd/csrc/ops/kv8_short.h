@@ -63,8 +63,9 @@ __global__ __launch_bounds__(K8S_WAVES * 64, 2) void kv8_short_kernel(
                                  &place))
     return;
   const int q_start = place.q_start, q_len = place.q_len;
-  const int ctx = place.seq_len - q_len, room = max_blocks * PF_BS;
-  const int seq_len = min(place.seq_len, room);
+  const int room = max_blocks * PF_BS;
+  const int ctx = max(place.seq_len, 0) - q_len;
+  const int seq_len = min(max(place.seq_len, 0), room);
   const int rows = q_len * G;
   const int row0 = place.lt * K8S_ROWS;
   const int rho = row0 + c32;

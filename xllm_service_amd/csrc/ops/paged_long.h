@@ -74,7 +74,8 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
                               n_seqs, G, lane, &place))
     return;
   const int seq = place.seq, lt = place.lt, q_start = place.q_start,
-            q_len = place.q_len, seq_len = place.seq_len;
+            q_len = place.q_len,
+            seq_len = CACHE8 ? max(place.seq_len, 0) : place.seq_len;
   const int ctx = seq_len - q_len;
   const int rows = q_len * G;
   // a table that ends before its sequence: what it does not have is not seen

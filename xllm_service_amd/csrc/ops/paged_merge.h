@@ -325,10 +325,12 @@ inline PagedMeet paged_meet(float* ws_ml, long rows, int parts) {
   return {reinterpret_cast<u64*>(ws_ml + 2 * rows * parts), (z ^ (z >> 31)) << 8};
 }
 
-// Tiles of kt keys that a prompt of `keys` of them walks at most
+// Tiles of kt keys that a prompt of `keys` of them walks at most. A length past 2^28, which
+// no table need hold, counts as that in plans: row tiles whose keys are split (at most 340)
+// times their tiles of keys stay below 2^31.
 template <bool MORE>
 XLLM_DEV int paged_walk(const PagedMore& x, int keys, int kt) {
-  const int n = (max(keys, 0) + kt - 1) / kt;
+  const int n = (min(max(keys, 0), 1 << 28) + kt - 1) / kt;
   return MORE && x.window > 0 ? min(n, (x.window + x.keep_first) / kt + 3) : n;
 }
 // Equal parts of a single prompt's rows, of at least four tiles

@@ -191,7 +191,10 @@ XLLM_DEV bool pf_longest(int b, int turn, const int* cu_q, const int* seq_lens,
     len = cu_q[lane + 1] - start;
     keys = seq_lens[lane];
   }
-  const int nt = (len * G + ROWS - 1) / ROWS, top = keys * G;
+  // (in fp32, to at most 10^9: lengths that tables need not hold would pass 32 bits, and an
+  // order needs no more)
+  const int nt = (len * G + ROWS - 1) / ROWS;
+  const int top = (int)fminf((float)max(keys, 0) * (float)G, 1e9f);
   const int most = __builtin_amdgcn_readlane(
       pf_scan<false>(nt > 0 ? top : INT_MIN), 63);
   const int total = __builtin_amdgcn_readlane(pf_scan<true>(nt), 63);
@@ -301,7 +304,7 @@ XLLM_DEV bool pf_parts(int b, int least, int most, int groups, int turn,
       auto turns = [&]() {
         const int now = chain(parts_of(per));
         if (groups > 1) return 2 * now;
-        const int seen = min(n, (max(keys - len / 2, 0) + PF_KT - 1) / PF_KT);
+        const int seen = min(n, paged_walk<false>(x, max(keys, 0) - len / 2, PF_KT));
         const int mean = __builtin_amdgcn_readlane(pf_scan<true>(nt * seen), 63);
         return now + (int)((float)now * mean / max(work, 1)) + (MORE ? 2 : 4);
       };
@@ -416,7 +419,7 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
       return;
   }
   const int seq = at.seq, lt = at.lt, q_start = at.q_start, q_len = at.q_len,
-            seq_len = at.seq_len;
+            seq_len = CACHE8 ? max(at.seq_len, 0) : at.seq_len;
   const int ctx = seq_len - q_len;
   const int rows = q_len * G;
   const int n_qheads = n_kv * G;
