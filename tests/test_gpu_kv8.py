@@ -128,6 +128,35 @@ def test_write_rows_at_any_address(offset):
     assert all(same(got.x[i], want.x[i]) for i in range(2))
 
 
+BIG = [3.3895313892515355e38, 3.3e38, 3.28e38, -3.3895313892515355e38, 3e38, 2.9e38,
+       1e38, 1.0]
+
+
+@pytest.mark.parametrize("heads,dim", [(3, 128), (2, 64)])
+def test_the_largest_values_stay_finite(heads, dim):
+    """448 times the largest scale passes fp32 and bf16: what would round to more
+    than 240 of it is 240, within half a step of e4m3 of what it was."""
+    cache = tuple(c.to(DEV) for c in ops.kv8_cache(4, heads, dim))
+    plain = ops.kv8_cache(4, heads, dim)
+    g = torch.Generator().manual_seed(1)
+    for slots in (list(range(16, 32)), [0], [1], [2, 3]):
+        x = torch.tensor(BIG)[torch.randint(len(BIG), (len(slots), heads, dim),
+                                            generator=g)].to(torch.bfloat16)
+        at = torch.tensor(slots)
+        ops.reshape_and_cache_kv8(x, x, *plain, at)
+        ops.reshape_and_cache_kv8(x.to(DEV), x.to(DEV), *cache, at.to(DEV))
+        for a, b in zip(cache, plain):
+            assert torch.equal(a.view(torch.uint8).cpu(), b.view(torch.uint8))
+        got = Cache(4, heads, dim).load(*cache)
+        for i in range(2):
+            y = got.values(i)[at // 16, :, at % 16]
+            assert (y.abs() < 2.0 ** 128 - 2.0 ** 119).all()     # bf16's largest
+            # (below 2^-6 of the scale a step is 2^-9 of it)
+            least = 2.0 ** -10 * got.scale[at // 16, :, i, None]
+            assert ((y - x.double()).abs()
+                    <= 2.0 ** -4 * x.double().abs() + least).all()
+
+
 # ---- tables ------------------------------------------------------------------
 @pytest.mark.parametrize("seqs,most_old,most_new,short", [
     (1, 0, 1, 0), (1, 100, 3, 0), (3, 40, 40, 0), (256, 300, 2, 0),
@@ -302,6 +331,27 @@ def test_values_that_are_not_finite_anywhere(token, heads, per, dim, width):
     got[token:, :, 33] = 0.0
     assert not got.isnan().any()
 
+
+
+@pytest.mark.parametrize("heads,per,dim,T,old,width", [
+    (64, 3, 128, 512, 0, 140), (2, 4, 128, 150, 5, 10), (2, 4, 128, 150, 5, 400),
+    (16, 4, 128, 600, 8, 38)])
+def test_the_largest_values_reach_rows_that_see_them(heads, per, dim, T, old, width):
+    """And no others, to which 0 times an infinity would bring a NaN."""
+    total = T + old
+    table, pages = layout([total], 3, 1, width)
+    cache = ops.kv8_cache(pages, heads, dim, DEV)
+    k, v = rows(total, heads, dim, 2), rows(total, heads, dim, 3)
+    token = T - 70
+    gv = part(v, heads, dim).clone()
+    gv[token + old:] = 3.3895313892515355e38
+    ops.reshape_and_cache_kv8(part(k, heads, dim), gv, *cache,
+                              ints(slots_of(table, [0], [total]), torch.long))
+    q = part(rows(T, heads * per, dim, 6), heads * per, dim)
+    got = ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints([0, T]),
+                                     ints([total]), 0.09)
+    assert got[:token].isfinite().all()
+    assert got[:token].abs().max() < 8.0
 
 # few rows over wide tables, whose keys are split over workgroups, and many over few keys
 ROWS = [(2, 4, 128, [9], [1200], 300), (2, 4, 128, [40, 3], [700, 90], 400),

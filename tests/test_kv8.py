@@ -52,6 +52,22 @@ def test_scale_borders():
         assert cache[1].float().isnan().sum() == 1
 
 
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+def test_the_largest_values_stay_finite(kind):
+    """448 * 2^120 is not: the largest values are 240 * 2^120."""
+    most = torch.finfo(kind).max
+    for big in (most, -most, 3.3e38, 3.2e38):
+        x = torch.full((3, 1, 64), big, dtype=kind)
+        cache = ops.kv8_cache(1, 1, 64)
+        ops.reshape_and_cache_kv8(x, x, *cache, torch.arange(3))
+        assert cache[2].tolist() == [[[2.0 ** 120] * 2]]
+        k = cache[0].float().transpose(2, 3).reshape(16, 64)[:3] * 2.0 ** 120
+        v = cache[1].float()[0, 0, :, :3] * 2.0 ** 120
+        for y in (k, v):
+            assert y.to(torch.bfloat16).isfinite().all()
+            assert ((y / x.flatten()[0].float() - 1).abs() <= 2.0 ** -4).all()
+
+
 @pytest.mark.parametrize("per", [1, 3])
 def test_attention_of_the_references(per):
     lens, new, dim = [0, 1, 17, 40], [2, 1, 5, 40], 64

@@ -298,6 +298,19 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
           }
       big = __builtin_amdgcn_readlane(pf_scan<false>(big), 63);
     }
+    // A scale of 2^120, which these have, takes 448 past what fp32 and bf16 hold: past 240 of
+    // it is 240, half a step off at most as any other
+    if (big > 0x7f70) {                    // uniform
+#pragma unroll
+      for (int i = 0; i < NP; i++)
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const unsigned a = x[i][c] >> (16 * e) & 0x7fff;
+            if (a > 0x7f70 && a < 0x7f80) x[i][c] -= (a - 0x7f70) << (16 * e);
+          }
+    }
     const bool anew = r.have & 1;
     const float fit = kv8_power(kv8_exponent(__int_as_float(big << 16)));
     const float now = anew ? fit : fmaxf(r.was, fit);

@@ -241,7 +241,7 @@ def reshape_and_cache_kv8(k, v, k_cache, v_cache, kv_scale, slot_mapping):
     offsets that none of them has become zero. Else its earlier tokens stay, and
     if the scale has to grow they are rounded to it once more (which changes only
     those that become subnormal). What is not finite is held as a NaN and does not
-    count for the scale."""
+    count for the scale; past 240 * 2^120, near the largest bf16, is that."""
     if kv_scale.is_cuda:
         _require_ext()
         _ops.reshape_and_cache_kv8(k, v, k_cache, v_cache, kv_scale,

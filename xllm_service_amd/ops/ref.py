@@ -162,6 +162,7 @@ def paged_attn_prefill(q, k_cache, v_cache, block_tables, cu_q, seq_lens, scale)
 
 # ---- paged cache held in 8 bits (csrc/ops/kv8.h) -----------------------------
 KV8_PAGE = 16
+KV8_LARGEST = 240.0 * 2.0 ** 120
 
 
 def extend_block_tables(block_tables, seq_lens, new_lens, free_blocks,
@@ -262,7 +263,9 @@ def reshape_and_cache_kv8(k, v, k_cache, v_cache, kv_scale, slot_mapping):
                 by = (was / now).reshape(KV, *[1] * (kept.dim() - 1))
                 raw[i][page] = (kept * by).to(f8).view(torch.uint8)
             kv_scale[page, :, i] = now
-            x = torch.where(x.isfinite(), x / now[None, :, None],
+            # (448 times the largest scale, 2^120, is not finite: 240 of it is)
+            x = torch.where(x.isfinite(), x.clamp(-KV8_LARGEST, KV8_LARGEST)
+                            / now[None, :, None],
                             torch.full_like(x, float("nan"))).to(f8)
             x = x.view(torch.uint8)
             for j, o in enumerate(offs):
