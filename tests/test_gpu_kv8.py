@@ -333,6 +333,41 @@ def test_values_that_are_not_finite_anywhere(token, heads, per, dim, width):
 
 
 
+UNUSED = [([40, 3], [700, 90], 2, 4, 128, 400), ([300, 7], [20, 0], 16, 4, 128, 21),
+          ([70] * 14, [3] * 14, 12, 3, 64, 6), ([600], [0], 24, 8, 128, 140),
+          ([300, 410], [100, 1700], 21, 8, 128, 140), ([100], [5], 2, 4, 128, 12),
+          ([150], [900], 2, 4, 64, 300), ([1] * 5, [0, 3, 40, 900, 31], 2, 12, 128, 60),
+          ([1] * 5, [0, 3, 40, 900, 31], 2, 4, 64, 60)]
+
+
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+@pytest.mark.parametrize("new,old,heads,per,dim,width", UNUSED)
+def test_scales_of_pages_that_are_not_used(new, old, heads, per, dim, width, what):
+    """Memory that nobody has cleared: page 0, which stands for what tables do not
+    have, and other pages of no sequence have scales that are not finite."""
+    lens = [n + o for n, o in zip(new, old)]
+    spare = sum(-(-n // 16) for n in lens)
+    for seed in range(99):
+        table, _ = layout(lens, spare, seed)
+        live = {int(p) for i, n in enumerate(lens) for p in table[i, :-(-n // 16)]}
+        if 0 not in live:
+            break
+    cache, want, table = filled(lens, heads, dim, seed, spare=spare, width=width)
+    cache[2][cache[2] == 2.0 ** 60] = what
+    assert not cache[2][0].isfinite().any()
+    for x in want.x:                             # (the oracle reads no such page)
+        x[[p for p in range(len(x)) if p not in live]] = 0.0
+    H, T = heads * per, sum(new)
+    q = part(rows(T, H, dim, 6), H, dim)
+    cu = [sum(new[:i]) for i in range(len(new) + 1)]
+    got = ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints(cu), ints(lens),
+                                     0.09)
+    close(got, q, want, table, cu, lens, 0.09, 2.0 ** -8)
+    if max(new) == 1:
+        got = ops.paged_attn_decode_kv8(q, *cache, table.to(DEV), ints(lens), 0.09)
+        close(got, q, want, table, cu, lens, 0.09, 2.0 ** -15)
+
+
 @pytest.mark.parametrize("heads,per,dim,T,old,width", [
     (64, 3, 128, 512, 0, 140), (2, 4, 128, 150, 5, 10), (2, 4, 128, 150, 5, 400),
     (16, 4, 128, 600, 8, 38)])

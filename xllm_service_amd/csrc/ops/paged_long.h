@@ -145,7 +145,8 @@ __global__ __launch_bounds__(512) void paged_attn_long_kernel(
       from_hi = (unsigned)(at >> 32);
       bytes = there ? PF_BS * D : 0;
       const float2 both = c8.scale[of];
-      size = __float_as_uint(half ? both.y : both.x);
+      // (behind the last page zeros are converted, by a scale that leaves them zeros)
+      size = there ? __float_as_uint(half ? both.y : both.x) : 0x3f800000u;
       asm volatile("" : "+v"(from_lo), "+v"(from_hi), "+v"(bytes), "+v"(size));
       return;
     }
