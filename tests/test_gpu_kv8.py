@@ -128,6 +128,34 @@ def test_write_rows_at_any_address(offset):
     assert all(same(got.x[i], want.x[i]) for i in range(2))
 
 
+@pytest.mark.parametrize("heads,dim", [(3, 128), (2, 64)])
+def test_write_twice_to_a_slot(heads, dim):
+    """The later one stays; the scale holds all of a page's new tokens, those that
+    do not stay among them, as it would after one call for each."""
+    cache = tuple(c.to(DEV) for c in ops.kv8_cache(7, heads, dim))
+    want = Cache(7, heads, dim)
+    for n, (slots, big) in enumerate([
+            ([2, 2], [300.0, 1.0]),
+            ([5, 3, 5, 4, 3], [1.0, 9.0, 2000.0, 1.0, 1.0]),
+            ([17, 17, 16, 19, 17], [50.0, 700.0, 1.0, 1.0, 1.0]),
+            ([32, -1, 32, 33, 32], [1.0, 1e5, 77.0, 1.0, 1.0]),
+            ([40, 40], [math.inf, 1.0]), ([41, 41, 41], [math.nan, 6e4, 1.0]),
+            # more of them than a wave looks over at once
+            ([64] + [65, 66] * 50 + [67], [1.0, 4000.0] + [1.0] * 100),
+            ([70] * 90 + [71], [1.0] * 30 + [1e6] + [1.0] * 60),
+            (list(range(80, 96)) * 5, [1.0] * 7 + [500.0] + [1.0] * 72)]):
+        k, v = (rows(len(slots), heads, dim, 2 * n + i) for i in range(2))
+        by = torch.tensor(big)[:, None]
+        gk, gv = (part((x.float() * by).to(torch.bfloat16), heads, dim)
+                  for x in (k, v))
+        ops.reshape_and_cache_kv8(gk, gv, *cache, ints(slots, torch.long))
+        want.write(gk, gv, slots)
+        got = Cache(7, heads, dim).load(*cache)
+        assert same(got.scale, want.scale), n
+        for i in range(2):
+            assert same(got.x[i], want.x[i]), (n, i)
+
+
 BIG = [3.3895313892515355e38, 3.3e38, 3.28e38, -3.3895313892515355e38, 3e38, 2.9e38,
        1e38, 1.0]
 

@@ -187,6 +187,8 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
     long at;                               // page and head
     float was;                             // scale
     unsigned have;                         // offsets with a new token
+    int gone;                              // largest finite value of this lane's of new
+                                           // tokens that later ones stand in the place of
   };
   auto place_of = [&](int i) { return 16 * (VAL ? NP * lane + i : lane + 64 * i); };
   auto load = [&](Run& r) {                // the next one
@@ -201,6 +203,7 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
     const int end = other == 0 ? 64 : __builtin_amdgcn_readfirstlane(__ffsll(other) - 1);
     const mask in = __ballot(page == id) & up & (end == 64 ? ~0ull : (1ull << end) - 1);
     int src = -1;                          // lane o < 16: offset o's last token
+    r.gone = 0;
     const int off0 = __builtin_amdgcn_readlane(off, j);
     const int n = __popcll(in);
     if (end < 64 && in == ((1ull << n) - 1) << j &&
@@ -211,7 +214,17 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
       auto place = [&](mask m, int o, int from) {
         for (; m != 0; m &= m - 1) {
           const int i = __builtin_amdgcn_readfirstlane(__ffsll(m) - 1);
-          if (lane == __builtin_amdgcn_readlane(o, i)) src = from + i;
+          const int at = __builtin_amdgcn_readlane(o, i);
+          const int t = __builtin_amdgcn_readlane(src, at);
+          if (t >= 0) {                    // uniform
+            const unsigned short* was = rows + t * stride + (long)head * D + NP * lane;
+#pragma unroll
+            for (int e = 0; e < NP; e++) {
+              const int a = was[e] & 0x7fff;
+              r.gone = max(r.gone, a < 0x7f80 ? a : 0);
+            }
+          }
+          if (lane == at) src = from + i;
         }
       };
       place(in, off, base);
@@ -283,10 +296,11 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
       for (int c = 0; c < 8; c++)
         two = __builtin_elementwise_max(
             two, __builtin_bit_cast(u16x2, x[i][c] & 0x7fff7fffu));
-    int big = __builtin_amdgcn_readlane(pf_scan<false>(max(two[0], two[1])), 63);
+    int big = __builtin_amdgcn_readlane(
+        pf_scan<false>(max(max((int)two[0], (int)two[1]), r.gone)), 63);
     const bool odd = big >= 0x7f80;        // uniform: not all finite
     if (odd) {
-      big = 0;
+      big = r.gone;
 #pragma unroll
       for (int i = 0; i < NP; i++)
 #pragma unroll

@@ -237,7 +237,8 @@ def reshape_and_cache_kv8(k, v, k_cache, v_cache, kv_scale, slot_mapping):
     same slot the later one stays.
 
     Where the token at offset 0 of a page is among them the page begins anew: its
-    scale is the least power of two whose multiple of 448 holds all of them, and
+    scale is the least power of two whose multiple of 448 holds all of them (of
+    two for the same slot, both), and
     offsets that none of them has become zero. Else its earlier tokens stay, and
     if the scale has to grow they are rounded to it once more (which changes only
     those that become subnormal). What is not finite is held as a NaN and does not
