@@ -166,7 +166,7 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
   if (before == 0) prev = -1;
   mask begins = ((2ull << window) - 2) & on;
   if (begins == 0) return;
-  if (!(on & 1) && base > 0) {             // only skipped ones: it is further up
+  if (__builtin_expect(!(on & 1) && base > 0, 0)) {   // only skipped ones: it is further up
     int found = -1;
     for (int end = base; end > 0 && found < 0; end -= 64) {
       const int p = page_of(slot_at(end - 64 + lane));
@@ -187,8 +187,7 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
     long at;                               // page and head
     float was;                             // scale
     unsigned have;                         // offsets with a new token
-    int gone;                              // largest finite value of this lane's of new
-                                           // tokens that later ones stand in the place of
+    int from, n;                           // first token, tokens
   };
   auto place_of = [&](int i) { return 16 * (VAL ? NP * lane + i : lane + 64 * i); };
   auto load = [&](Run& r) {                // the next one
@@ -203,38 +202,35 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
     const int end = other == 0 ? 64 : __builtin_amdgcn_readfirstlane(__ffsll(other) - 1);
     const mask in = __ballot(page == id) & up & (end == 64 ? ~0ull : (1ull << end) - 1);
     int src = -1;                          // lane o < 16: offset o's last token
-    r.gone = 0;
+    r.from = base + j;
     const int off0 = __builtin_amdgcn_readlane(off, j);
-    const int n = __popcll(in);
-    if (end < 64 && in == ((1ull << n) - 1) << j &&
-        (__ballot(off == off0 + lane - j) & in) == in) {
+    r.n = __popcll(in);
+    if (__builtin_expect(end < 64 && in == ((1ull << r.n) - 1) << j &&
+                             (__ballot(off == off0 + lane - j) & in) == in, 1)) {
       // tokens one after the other
-      if (lane >= off0 && lane < off0 + n) src = base + j + lane - off0;
+      if (lane >= off0 && lane < off0 + r.n) src = base + j + lane - off0;
     } else {
-      auto place = [&](mask m, int o, int from) {
+      mask m = in;                         // of the 64 tokens from b on
+      int o = off, b = base;
+      for (bool last = end < 64;;) {
         for (; m != 0; m &= m - 1) {
           const int i = __builtin_amdgcn_readfirstlane(__ffsll(m) - 1);
           const int at = __builtin_amdgcn_readlane(o, i);
-          const int t = __builtin_amdgcn_readlane(src, at);
-          if (t >= 0) {                    // uniform
-            const unsigned short* was = rows + t * stride + (long)head * D + NP * lane;
-#pragma unroll
-            for (int e = 0; e < NP; e++) {
-              const int a = was[e] & 0x7fff;
-              r.gone = max(r.gone, a < 0x7f80 ? a : 0);
-            }
-          }
-          if (lane == at) src = from + i;
+          if (lane == at) src = b + i;
         }
-      };
-      place(in, off, base);
-      for (int b = base + 64; end == 64 && b < n_tokens; b += 64) {
+        if (last) break;
+        b += 64;
+        if (b >= n_tokens) break;
         const long s = slot_at(b + lane);
         const int p = page_of(s);
         const mask out = __ballot(p >= 0 && p != id);
-        const mask m = __ballot(p == id);
-        place(out == 0 ? m : m & ((out & -out) - 1), (int)(s & (KV8_PAGE - 1)), b);
-        if (out != 0) break;
+        m = __ballot(p == id);
+        o = (int)(s & (KV8_PAGE - 1));
+        if (out != 0) {
+          m &= (out & -out) - 1;
+          last = true;
+        }
+        r.n += __popcll(m);
       }
     }
     r.have = (unsigned)__ballot(src >= 0);
@@ -296,11 +292,10 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
       for (int c = 0; c < 8; c++)
         two = __builtin_elementwise_max(
             two, __builtin_bit_cast(u16x2, x[i][c] & 0x7fff7fffu));
-    int big = __builtin_amdgcn_readlane(
-        pf_scan<false>(max(max((int)two[0], (int)two[1]), r.gone)), 63);
+    int big = __builtin_amdgcn_readlane(pf_scan<false>(max(two[0], two[1])), 63);
     const bool odd = big >= 0x7f80;        // uniform: not all finite
-    if (odd) {
-      big = r.gone;
+    if (__builtin_expect(odd, 0)) {
+      big = 0;
 #pragma unroll
       for (int i = 0; i < NP; i++)
 #pragma unroll
@@ -312,18 +307,25 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
           }
       big = __builtin_amdgcn_readlane(pf_scan<false>(big), 63);
     }
-    // A scale of 2^120, which these have, takes 448 past what fp32 and bf16 hold: past 240 of
-    // it is 240, half a step off at most as any other
-    if (big > 0x7f70) {                    // uniform
-#pragma unroll
-      for (int i = 0; i < NP; i++)
-#pragma unroll
-        for (int c = 0; c < 8; c++)
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const unsigned a = x[i][c] >> (16 * e) & 0x7fff;
-            if (a > 0x7f70 && a < 0x7f80) x[i][c] -= (a - 0x7f70) << (16 * e);
+    // tokens that later ones stand in the place of count too
+    if (__builtin_expect(r.n > __popc(r.have), 0)) {
+      const int id = (int)((unsigned long)r.at / (unsigned)n_kv);
+      mask out = 0;
+      for (int b = r.from; b < n_tokens && out == 0; b += 64) {
+        const int p = page_of(slot_at(b + lane));
+        out = __ballot(p >= 0 && p != id);
+        mask m = __ballot(p == id);
+        if (out != 0) m &= (out & -out) - 1;
+        for (; m != 0; m &= m - 1) {
+          const long t = b + __builtin_amdgcn_readfirstlane(__ffsll(m) - 1);
+          const unsigned short* row = rows + t * stride + (long)head * D;
+          for (int e = lane; e < D; e += 64) {
+            const int a = row[e] & 0x7fff;
+            big = max(big, a < 0x7f80 ? a : 0);
           }
+        }
+      }
+      big = __builtin_amdgcn_readlane(pf_scan<false>(big), 63);
     }
     const bool anew = r.have & 1;
     const float fit = kv8_power(kv8_exponent(__int_as_float(big << 16)));
@@ -343,6 +345,16 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
                         __uint_as_float(a & 0xffff0000u) * by,
                         __uint_as_float(b << 16) * by,
                         __uint_as_float(b & 0xffff0000u) * by);
+      }
+      // 448 times the largest scale is past what fp32 and bf16 hold: what has become more
+      // than 240 of it is 240, half a step off at most as any other
+      if (__builtin_expect(__builtin_amdgcn_readfirstlane(now >= 0x1p120f), 0)) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          unsigned far = ((u[c] & 0x7f7f7f7fu) + 0x08080808u) & 0x80808080u & ~kv8_nan(u[c]);
+          far = (far >> 7) * 0x7fu;
+          u[c] = (u[c] & ~far) | (0x77777777u & far);
+        }
       }
       if (!anew) {                         // uniform
         if (!keep) {
@@ -370,14 +382,11 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
   Run a, b;
   load(a);
   for (;;) {
-    const bool two = begins != 0;
-    if (two) load(b);
-    store(a);
-    if (!two) break;
     const bool more = begins != 0;
-    if (more) load(a);
-    store(b);
+    if (more) load(b);
+    store(a);
     if (!more) break;
+    a = b;
   }
 }
 
