@@ -156,6 +156,32 @@ def test_write_twice_to_a_slot(heads, dim):
             assert same(got.x[i], want.x[i]), (n, i)
 
 
+@pytest.mark.parametrize("room", [50, 63, 64, 65, 1023, 1100, 8192, 20000])
+def test_write_of_padded_rows(room):
+    """Few tokens anywhere among rows without a slot: in front, behind, and a page's
+    first and last ones far apart."""
+    heads, dim = 1, 64
+    k, v = (part(rows(room, heads, dim, i), heads, dim) for i in range(2))
+    page = [*range(16, 30)]
+    for where in (list(range(14)), list(range(room - 14, room)),
+                  [0, *range(room - 13, room)], [*range(13), room - 1],
+                  [room // 14 * i for i in range(14)], [*range(20, 33), room - 9]):
+        cache = tuple(c.to(DEV) for c in ops.kv8_cache(3, heads, dim))
+        want = Cache(3, heads, dim)
+        slots = [-1] * room
+        for at, s in zip(where, page):
+            slots[at] = s
+        if where[0] > 0:
+            slots[where[0] - 1] = 40         # another page's, right before it
+        if where[-1] < room - 3:
+            slots[room - 2] = 5
+        ops.reshape_and_cache_kv8(k, v, *cache, ints(slots, torch.long))
+        want.write(k, v, slots)
+        got = Cache(3, heads, dim).load(*cache)
+        assert same(got.scale, want.scale), where
+        assert all(same(got.x[i], want.x[i]) for i in range(2)), where
+
+
 BIG = [3.3895313892515355e38, 3.3e38, 3.28e38, -3.3895313892515355e38, 3e38, 2.9e38,
        1e38, 1.0]
 

@@ -153,6 +153,21 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
     const long s = slots[t];
     return (unsigned long)s < (unsigned long)n_blocks * KV8_PAGE ? s : -1L;
   };
+  // Whether one of FAR tokens from t on has a slot, by loads that are waited for together:
+  // padding is long and has none. Us, 64 at a time | so, 8 heads of 128: 10 tokens in front of
+  // padding to 8192 rows 33 | 11.4 (to 256, by 64 at a time, 5.5 | 6.4), to 65 k 238 | 52, to 2^20 5630 | 732.
+  constexpr int FAR = 1024;
+  auto any_from = [&](int t) {
+    long s[FAR / 64];
+#pragma unroll
+    for (int i = 0; i < FAR / 64; i++)
+      s[i] = slots[min(max(t + 64 * i + lane, 0), n_tokens - 1)];
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < FAR / 64; i++)
+      any |= (unsigned long)s[i] < (unsigned long)n_blocks * KV8_PAGE;
+    return __any(any);                     // (more than asked for at the ends, if any)
+  };
   auto page_of = [](long slot) { return slot < 0 ? -1 : (int)(slot / KV8_PAGE); };
   // lane i has token base + i: the window, one before it, and what follows
   const int base = (int)blockIdx.x * window - 1;
@@ -169,6 +184,10 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
   if (__builtin_expect(!(on & 1) && base > 0, 0)) {   // only skipped ones: it is further up
     int found = -1;
     for (int end = base; end > 0 && found < 0; end -= 64) {
+      if (end > FAR / 2 && !any_from(end - FAR)) {
+        end += 64 - FAR;
+        continue;
+      }
       const int p = page_of(slot_at(end - 64 + lane));
       const mask any = __ballot(p >= 0);
       if (any != 0) found = __builtin_amdgcn_readlane(p, 63 - __clzll(any));
@@ -177,6 +196,14 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
   }
   begins &= __ballot(page != prev);
   if (begins == 0) return;
+
+  // where the last of these runs goes on behind the 64 tokens, if it may and many follow
+  int next = base + 64;
+  if (__builtin_expect(
+          n_tokens - next > FAR / 2 &&
+              __builtin_amdgcn_readlane(page, 63 - __clzll(on)) ==
+                  __builtin_amdgcn_readlane(page, 63 - __clzll(begins)), 0))
+    while (next < n_tokens && !any_from(next)) next += FAR;
 
   struct Run {                             // on its way
     unsigned raw[8 * NP];                  // this lane's new values, in bf16: keys, 16
@@ -219,7 +246,7 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
           if (lane == at) src = b + i;
         }
         if (last) break;
-        b += 64;
+        b = max(b + 64, next);
         if (b >= n_tokens) break;
         const long s = slot_at(b + lane);
         const int p = page_of(s);
