@@ -442,6 +442,27 @@ def test_the_largest_values_reach_rows_that_see_them(heads, per, dim, T, old, wi
     assert got[:token].isfinite().all()
     assert got[:token].abs().max() < 8.0
 
+
+@pytest.mark.parametrize("heads,per,dim", [(2, 4, 128), (3, 1, 64), (1, 7, 128)])
+def test_parts_without_keys_beside_values_that_are_not_finite(heads, per, dim):
+    """Row tiles that see fewer tiles of keys than they have parts, by turns with
+    calls whose every value is a NaN, which leave LDS full of what they noted."""
+    T, width = 260, 400
+    cache, want, table = filled([T], heads, dim, 3, width=width)
+    bad = [c.clone() for c in cache]
+    bad[1].view(torch.uint8).fill_(0x7f)
+    q = part(rows(T, heads * per, dim, 6), heads * per, dim)
+    for _ in range(4):
+        got = ops.paged_attn_prefill_kv8(q, *bad, table.to(DEV), ints([0, T]),
+                                         ints([T]), 0.09)
+        assert got.isnan().all()
+        got = ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints([0, T]),
+                                         ints([T]), 0.09)
+        close(got, q, want, table, [0, T], [T], 0.09, 2.0 ** -8)
+        got = ops.paged_attn_prefill_kv8(q, *bad, table.to(DEV), ints([0, T]),
+                                         ints([40]), 0.09)
+        assert (got[:T - 40] == 0).all() and got[T - 40:].isnan().all()
+
 # few rows over wide tables, whose keys are split over workgroups, and many over few keys
 ROWS = [(2, 4, 128, [9], [1200], 300), (2, 4, 128, [40, 3], [700, 90], 400),
         (1, 8, 64, [30], [900], 260), (16, 4, 128, [80] * 9, [0] * 9, 8),

@@ -730,9 +730,10 @@ __global__ __launch_bounds__(KG * 256, 2) void paged_attn_rows_kernel(
       }
   }
   if constexpr (CACHE8) {
-    // values that are NaNs, zeros in their tiles: for the rows that see them
-    const int from = first8 * PF_KT;
-    for (int e = 0; e < EDGES; e++) {
+    // values that are NaNs, zeros in their tiles: for the rows that see them. (Without
+    // tiles there was no barrier behind what others of the waves have noted.)
+    const int from = first8 * PF_KT, edges = p_begin < i_end ? EDGES : 0;
+    for (int e = 0; e < edges; e++) {
       unsigned long long sees = limit - from >= PF_KT * (e + 1) ? ~0ull
           : (1ull << min(max(limit - from - PF_KT * e, 0), PF_KT - 1)) - 1;
       bool any = false;
