@@ -96,6 +96,34 @@ def test_attention_of_the_references(per):
     assert torch.allclose(got.double(), want, atol=1e-5)
 
 
+def test_values_that_are_not_finite():
+    """A NaN among a sequence's values is seen by the rows that see it, and by no
+    others; nor is what a page holds behind its last token."""
+    lens, dim = [40, 70], 64
+    table, pages = layout(lens, 2, 8)
+    cache = ops.kv8_cache(pages, 2, dim)
+    slots = slots_of(table, [0, 0], lens)
+    k, v = rows(len(slots), 2, dim, 2), rows(len(slots), 2, dim, 3)
+    v[40 + 20, 1, 5] = math.inf                   # the second one's token 20
+    k[40 + 30, 0, 7] = math.nan                   # and 30
+    ops.reshape_and_cache_kv8(k, v, *cache, torch.tensor(slots))
+    cache[1].view(torch.uint8)[table[0, 2], :, :, 8:] = 0x7f
+    q = rows(110, 4, dim, 4).float()
+    got = ops.paged_attn_prefill_kv8(q, *cache, table, torch.tensor([0, 40, 110]).int(),
+                                     torch.tensor(lens).int(), 0.1)
+    assert got[:60].isfinite().all()
+    assert got[60:, 2:, 5].isnan().all()
+    got[60:, 2:, 5] = 0.0
+    assert got[:70].isfinite().all() and got[:, 2:].isfinite().all()
+    assert got[70:, :2].isnan().all()
+    got = ops.paged_attn_decode_kv8(q[:2], *cache, table,
+                                    torch.tensor([40, 20]).int(), 0.1)
+    assert got.isfinite().all()
+    got = ops.paged_attn_decode_kv8(q[:2], *cache, table,
+                                    torch.tensor([40, 21]).int(), 0.1)
+    assert got[1, 2:, 5].isnan().all() and got[0].isfinite().all()
+
+
 def plan_of(table, old, new, free, room):
     """Token by token, page by page."""
     table = [list(map(int, r)) for r in table]

@@ -311,7 +311,11 @@ def paged_attn_prefill_kv8(q, k_cache, v_cache, kv_scale, block_tables, cu_q,
             z = (q[q0:q1, h].float() @ kk.T) * scale
             p = torch.softmax(z.masked_fill(~seen, float("-inf")), -1)
             p = torch.where(seen.any(-1, keepdim=True), p, 0.0)
-            out[q0:q1, h] = (p @ vv).to(q.dtype)
+            nan = vv.isnan()
+            o = p @ vv.masked_fill(nan, 0.0)
+            if nan.any():        # 0 times one, of a row that does not see it, is one
+                o[(seen.float() @ nan.float()) > 0] = float("nan")
+            out[q0:q1, h] = o.to(q.dtype)
     return out
 
 
