@@ -124,6 +124,25 @@ def test_values_that_are_not_finite():
     assert got[1, 2:, 5].isnan().all() and got[0].isfinite().all()
 
 
+def test_attention_reads_the_pages_of_its_tables(monkeypatch):
+    """Not the pool: what is made of pages in 32 bits is as large as the sequences."""
+    from xllm_service_amd.ops import ref
+    lens, dim = [40, 0, 70], 64
+    table, pages = layout(lens, 300, 8)
+    cache = ops.kv8_cache(pages, 2, dim)
+    most, plain = [], ref.kv8_values
+
+    def values(k_cache, v_cache, kv_scale):
+        most.append(k_cache.shape[0])
+        return plain(k_cache, v_cache, kv_scale)
+    monkeypatch.setattr(ref, "kv8_values", values)
+    n = torch.tensor(lens).int()
+    ops.paged_attn_decode_kv8(rows(3, 4, dim, 4), *cache, table, n, 0.1)
+    ops.paged_attn_prefill_kv8(rows(7, 4, dim, 4), *cache, table,
+                               torch.tensor([0, 2, 4, 7]).int(), n, 0.1)
+    assert most and max(most) <= 5
+
+
 def plan_of(table, old, new, free, room):
     """Token by token, page by page."""
     table = [list(map(int, r)) for r in table]

@@ -293,8 +293,7 @@ def paged_attn_prefill_kv8(q, k_cache, v_cache, kv_scale, block_tables, cu_q,
     if cu_q.dtype != torch.int32 or cu_q.dim() != 1 or cu_q.shape[0] < 1:
         raise RuntimeError("kv8: cu_q must be int32")
     _kv8_check_attention(q, cache, block_tables, seq_lens, cu_q.shape[0] - 1)
-    k, v = kv8_values(*cache)
-    B, KV, _, D = k.shape
+    B, KV, D = kv8_shape(*cache)
     G = q.shape[1] // KV
     out = torch.zeros_like(q) if out is None else out
     cu = cu_q.tolist()
@@ -303,11 +302,16 @@ def paged_attn_prefill_kv8(q, k_cache, v_cache, kv_scale, block_tables, cu_q,
         L = max(min(total, block_tables.shape[1] * KV8_PAGE), 0)
         ids = block_tables[s, :-(-L // KV8_PAGE)].long()
         ids = torch.where((ids >= 0) & (ids < B), ids, 0)
+        if L == 0:
+            out[q0:q1] = 0
+            continue
+        # of the table's pages alone: a pool in 32 bits is four times what it takes
+        k, v = kv8_values(*(c.view(torch.uint8)[ids].view(c.dtype) for c in cache))
         seen = torch.arange(L) <= (total - (q1 - q0)
                                    + torch.arange(q1 - q0))[:, None]
         for h in range(q.shape[1]):
-            kk = k[ids, h // G].reshape(-1, D)[:L]
-            vv = v[ids, h // G].reshape(-1, D)[:L]
+            kk = k[:, h // G].reshape(-1, D)[:L]
+            vv = v[:, h // G].reshape(-1, D)[:L]
             z = (q[q0:q1, h].float() @ kk.T) * scale
             p = torch.softmax(z.masked_fill(~seen, float("-inf")), -1)
             p = torch.where(seen.any(-1, keepdim=True), p, 0.0)
