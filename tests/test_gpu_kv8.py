@@ -848,6 +848,40 @@ def test_refusals():
     no(e, tab.expand(4, 3), lens, lens, lens, 4)
 
 
+@pytest.mark.parametrize("kind", ["fp8", None])
+@pytest.mark.parametrize("tier", ["dram", "ssd"])
+def test_engine_swaps_blocks(kind, tier, tmp_path):
+    """Blocks out to the host or a file and back into others: the same bytes, those
+    beside them untouched."""
+    from xllm_service_amd.engine.engine import LLMEngine
+    from xllm_service_amd.engine.sampling import SamplingParams
+    from xllm_service_amd.engine.sequence import Sequence
+    eng = LLMEngine("llama-tiny", device="cuda:0", max_kv_blocks=32, seed=3,
+                    max_num_seqs=4, max_model_len=256, enable_graphs=False,
+                    kv_cache_dtype=kind, enable_prefix_caching=False,
+                    swap_space_mb=0 if tier == "ssd" else 64,
+                    ssd_swap_dir=str(tmp_path / "spool"))
+    assert (eng.cpu_block_manager is None) == (tier == "ssd")
+    eng.generate([[5, 9, 2, 7] * 30, list(range(40, 100))],
+                 SamplingParams(max_tokens=20, ignore_eos=True))
+    tensors = eng.runner.paged_tensors()
+    was = [c.clone() for c in tensors]
+    assert all((c != 0).any() for c in was)
+    seq = Sequence(request_id="s", prompt_token_ids=[1] * 70,
+                   params=SamplingParams())
+    seq.block_table = out = eng.block_manager.allocate_raw(5)
+    seq.block_table = out = [out[i] for i in (3, 0, 1, 4, 2)]
+    seq.cpu_block_table = eng._swap_out(seq)
+    hold = eng.block_manager.allocate_raw(3)
+    eng._swap_in(seq)
+    into = seq.block_table
+    assert not set(into) & set(out + hold)
+    rest = [i for i in range(32) if i not in into]
+    for c, w in zip(tensors, was):
+        assert torch.equal(c[into], w[out])
+        assert torch.equal(c[rest], w[rest])
+
+
 @pytest.mark.parametrize("model", ["llama-tiny", "llama-debug-128", "opt-125m"])
 def test_engine(model):
     """The engine over 8-bit pages: captured decode steps are the eager ones."""

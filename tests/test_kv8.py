@@ -323,6 +323,38 @@ def test_engine_first_logits():
     assert 0 < diff < bound
 
 
+@pytest.mark.parametrize("tier", ["dram", "ssd"])
+def test_engine_swaps(tier, tmp_path):
+    """Preempted sequences' pages go to the host's memory or to files, and come back
+    with their scales: the tokens are those of a pool that holds all of them."""
+    import os
+
+    from xllm_service_amd.engine.sampling import SamplingParams
+    g = torch.Generator().manual_seed(17)
+    prompts = [torch.randint(0, 500, (60,), generator=g).tolist() for _ in range(2)]
+    sp = SamplingParams(max_tokens=8, ignore_eos=True)
+    want = engine(max_kv_blocks=64, kv_cache_dtype="fp8",
+                  enable_prefix_caching=False).generate(prompts, sp)
+    spool = str(tmp_path / "spool")
+    kw = dict(swap_space_mb=0, ssd_swap_dir=spool) if tier == "ssd" else {}
+    # two sequences of four blocks, each of which needs a fifth
+    eng = engine(max_kv_blocks=9, kv_cache_dtype="fp8",
+                 enable_prefix_caching=False, **kw)
+    assert (eng.cpu_block_manager is None) == (tier == "ssd")
+    assert eng.generate(prompts, sp) == want
+    assert eng.scheduler.num_swap_outs > 0 and eng.scheduler.num_swap_ins > 0
+    assert eng.block_manager.num_free == eng.block_manager.num_blocks
+    if tier == "ssd":
+        assert os.listdir(spool) == []
+    else:
+        assert eng.cpu_block_manager.num_free == eng.cpu_block_manager.num_blocks
+
+
+def test_engine_of_several_ranks_does_not_swap(tmp_path):
+    with pytest.raises(ValueError, match="several ranks"):
+        engine(kv_cache_dtype="fp8", tp_size=2, ssd_swap_dir=str(tmp_path))
+
+
 @pytest.mark.parametrize("heads,kv_heads,good", [
     (32, 2, True), (34, 2, False), (17, 1, False)])
 def test_query_heads_per_key_head(heads, kv_heads, good):

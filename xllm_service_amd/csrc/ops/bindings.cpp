@@ -853,8 +853,10 @@ void swap_blocks(torch::Tensor dst_cache, torch::Tensor src_cache,
                  std::vector<long> src_blocks, std::vector<long> dst_blocks) {
   TORCH_CHECK(src_blocks.size() == dst_blocks.size());
   TORCH_CHECK(src_cache.element_size() == dst_cache.element_size());
-  const long numel =
-      (long)src_cache.size(1) * src_cache.size(2) * src_cache.size(3);
+  TORCH_CHECK(src_cache.sizes().slice(1) == dst_cache.sizes().slice(1) &&
+                  src_cache.is_contiguous() && dst_cache.is_contiguous(),
+              "swap_blocks: blocks of two shapes");
+  const long numel = src_cache.numel() / std::max<long>(src_cache.size(0), 1);
   const long bytes = numel * src_cache.element_size();
   char* dst = reinterpret_cast<char*>(dst_cache.data_ptr());
   const char* src = reinterpret_cast<const char*>(src_cache.data_ptr());

@@ -104,8 +104,12 @@ class LLMEngine:
                  seed: int = 0):
         # kv_cache_dtype: "fp8" keeps keys and values of a dense decoder in 8
         # bits with a scale for each block and head: half the bytes, so twice the
-        # blocks in the same memory. Preempted sequences recompute, and blocks
-        # move between workers as bytes.
+        # blocks in the same memory. Blocks move between workers as bytes.
+        # (The other ranks of a group do not replay swaps: sequences with pages
+        # of 8 bits recompute there.)
+        ranks_kv8 = kv_cache_dtype is not None and tp_size > 1
+        if ranks_kv8 and ssd_swap_dir:
+            raise ValueError("an 8-bit cache of several ranks is not swapped")
         # model_name: a preset, or a folder holding config.json + safetensors
         self.cfg: ModelConfig = get_config(model_name)
         # tensor parallelism: every rank of the TP group builds its shard;
@@ -150,8 +154,7 @@ class LLMEngine:
                 and dtype != torch.bfloat16:
             raise ValueError("an 8-bit cache takes bf16 models on a GPU")
         specs = ModelRunner.specs_for(self.model, self.cfg, kv_cache_dtype)
-        custom_cache = hasattr(self.model, "cache_specs") \
-            or kv_cache_dtype is not None
+        custom_cache = hasattr(self.model, "cache_specs") or ranks_kv8
         from .cache_spec import needs_state_slots
         # recurrent-state layers: one slot per live sequence. Such a state
         # cannot be rebuilt from shared prefix blocks, so prefix reuse is
@@ -291,10 +294,9 @@ class LLMEngine:
         if cbm is None or cbm.num_free < n:
             return self._ssd_swap_out(seq)  # dram full -> ssd tier
         cpu_blocks = cbm.allocate_raw(n)
-        for (kc, vc), (ck, cv) in zip(self.runner.kv_caches,
-                                      self.runner.cpu_kv_caches):
-            xops.swap_blocks(ck, kc, seq.block_table, cpu_blocks)
-            xops.swap_blocks(cv, vc, seq.block_table, cpu_blocks)
+        for c, host in zip(self.runner.paged_tensors(),
+                           self.runner.cpu_kv_caches):
+            xops.swap_blocks(host, c, seq.block_table, cpu_blocks)
         if self.device.type == "cuda":
             torch.cuda.synchronize(self.device)
         return cpu_blocks
@@ -324,10 +326,9 @@ class LLMEngine:
             return
         n = len(seq.cpu_block_table)
         gpu_blocks = self.block_manager.allocate_raw(n)
-        for (kc, vc), (ck, cv) in zip(self.runner.kv_caches,
-                                      self.runner.cpu_kv_caches):
-            xops.swap_blocks(kc, ck, seq.cpu_block_table, gpu_blocks)
-            xops.swap_blocks(vc, cv, seq.cpu_block_table, gpu_blocks)
+        for c, host in zip(self.runner.paged_tensors(),
+                           self.runner.cpu_kv_caches):
+            xops.swap_blocks(c, host, seq.cpu_block_table, gpu_blocks)
         if self.device.type == "cuda":
             torch.cuda.synchronize(self.device)
         self._free_cpu_blocks(seq)

@@ -113,16 +113,12 @@ class ModelRunner:
         return out
 
     def alloc_cpu_caches(self, num_cpu_blocks: int):
-        """Pinned host-DRAM tier for KV swapping."""
-        n_kv = self.kv_caches[0][0].shape[1]
+        """Pinned host-DRAM tier for KV swapping: a tensor for each of
+        paged_tensors()."""
         pin = self.device.type == "cuda"
         self.cpu_kv_caches = [
-            (torch.zeros(num_cpu_blocks, n_kv, BLOCK_SIZE, self.cfg.head_dim,
-                         dtype=self.dtype, pin_memory=pin),
-             torch.zeros(num_cpu_blocks, n_kv, BLOCK_SIZE, self.cfg.head_dim,
-                         dtype=self.dtype, pin_memory=pin))
-            for _ in range(self.cfg.num_layers)
-        ]
+            torch.zeros(num_cpu_blocks, *c.shape[1:], dtype=c.dtype,
+                        pin_memory=pin) for c in self.paged_tensors()]
 
     @staticmethod
     def kv_cache_blocks_for(cfg: ModelConfig, device: torch.device,
