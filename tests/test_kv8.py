@@ -323,6 +323,29 @@ def test_engine_first_logits():
     assert 0 < diff < bound
 
 
+@pytest.mark.parametrize("kind", [None, "fp8"])
+def test_engine_imports_blocks_of_its_cache(kind):
+    """Too few bytes change nothing; an 8-bit cache takes those of its blocks alone,
+    others what is behind them as well, as they did."""
+    eng = engine(max_kv_blocks=8, kv_cache_dtype=kind)
+    tensors = eng.runner.paged_tensors()
+    for i, c in enumerate(tensors):
+        c.fill_(1 + i % 3)
+    data = eng.export_block_bytes([1, 2])
+    for c in tensors:
+        c.fill_(7)
+    with pytest.raises(ValueError, match="another cache"):
+        eng.import_block_bytes([3, 4], data[:-1])
+    assert all((c == 7).all() for c in tensors)
+    if kind is not None:
+        with pytest.raises(ValueError, match="another cache"):
+            eng.import_block_bytes([3, 4], data + b"x")
+        assert all((c == 7).all() for c in tensors)
+    eng.import_block_bytes([3, 4], data if kind else data + b"beyond")
+    for i, c in enumerate(tensors):
+        assert (c[3:5] == 1 + i % 3).all() and (c[:3] == 7).all()
+
+
 @pytest.mark.parametrize("tier", ["dram", "ssd"])
 def test_engine_swaps(tier, tmp_path):
     """Preempted sequences' pages go to the host's memory or to files, and come back

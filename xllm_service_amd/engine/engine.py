@@ -637,7 +637,10 @@ class LLMEngine:
         off = 0
         need = sum(len(block_ids) * c[0].numel() * c.element_size()
                    for c in self.runner.paged_tensors())
-        if need != len(data):
+        # (bytes behind the blocks are of no matter but where they say that the
+        # cache they come from holds more than 8 bits)
+        if need > len(data) or (self.kv_cache_dtype is not None
+                                and need != len(data)):
             raise ValueError("the blocks are another cache's")
         for c in self.runner.paged_tensors():
             per = len(block_ids) * c[0].numel() * c.element_size()
