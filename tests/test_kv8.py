@@ -346,6 +346,50 @@ def test_engine_imports_blocks_of_its_cache(kind):
         assert (c[3:5] == 1 + i % 3).all() and (c[:3] == 7).all()
 
 
+@pytest.fixture
+def anyio_backend():
+    return "asyncio"
+
+
+@pytest.mark.anyio
+@pytest.mark.parametrize("kinds", [("fp8", "fp8"), ("fp8", None), (None, "fp8")])
+async def test_workers_of_a_pair(kinds):
+    """Prompt and tokens on two workers: blocks of 8 bits move between equal caches; of
+    a pair of different ones the request ends before its prompt is computed."""
+    from tests.test_service_integration import (http_client, make_master,
+                                                wait_for, worker_kwargs)
+    from xllm_service_amd.engine.worker import Worker
+    master = make_master(policy="RR")
+    await master.start(serve_http=False)
+    pair = [Worker(name, role, **worker_kwargs(
+        master, engine_kwargs=dict(seed=11, kv_cache_dtype=kind)))
+        for name, role, kind in zip(("p0", "d0"), ("PREFILL", "DECODE"), kinds)]
+    try:
+        for w in pair:
+            await w.start()
+        await wait_for(lambda: master.scheduler.has_available_instances()
+                       and "d0" in pair[0].peers and "p0" in pair[1].peers)
+        assert pair[0].peers["d0"].kv_cache_dtype == (kinds[1] or "")
+        client = await http_client(master)
+        r = await client.post("/v1/completions", json={
+            "model": "llama-tiny", "prompt": list(range(50, 90)),
+            "max_tokens": 6, "temperature": 0.0, "ignore_eos": True})
+        await client.aclose()
+        if kinds[0] == kinds[1]:
+            assert r.status_code == 200, r.text
+            assert r.json()["usage"]["completion_tokens"] == 6
+        else:
+            assert r.status_code != 200 and "cache" in r.text, r.text
+            assert pair[0].engine.stats.steps == 0
+            for w in pair:
+                bm = w.engine.block_manager
+                assert bm.num_free == bm.num_blocks
+    finally:
+        for w in pair:
+            await w.stop()
+        await master.stop()
+
+
 @pytest.mark.parametrize("tier", ["dram", "ssd"])
 def test_engine_swaps(tier, tmp_path):
     """Preempted sequences' pages go to the host's memory or to files, and come back

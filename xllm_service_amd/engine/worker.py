@@ -206,6 +206,9 @@ class Worker:
     def _regkey(self) -> str:
         return KEY_INSTANCE[self.itype] + self.name
 
+    def _cache_kind(self) -> str:
+        return getattr(self.engine, "kv_cache_dtype", None) or ""
+
     def meta(self) -> InstanceMetaInfo:
         dev = -1
         if self.engine is not None and self.engine.device.type == "cuda":
@@ -219,6 +222,7 @@ class Worker:
             if self.engine else 0,
             dp_size=1,
             block_size=16, model=self.model,
+            kv_cache_dtype=self._cache_kind(),
             incarnation_id=self.incarnation,
             k_cache_ids=list(range(self.engine.cfg.num_layers))
             if self.engine else [],
@@ -393,17 +397,27 @@ class Worker:
                                            multimodal)
             return
         sp = params_from_dict(params)
-        if self.engine is not None and (
-                not token_ids
-                or len(token_ids) >= self.engine.max_model_len):
+        error = None
+        if self.engine is not None:
+            decode_name = routing.get("decode_name")
+            peer = None
+            if self.itype == InstanceType.PREFILL and decode_name != self.name:
+                peer = self.peers.get(decode_name)
+            if not token_ids:
+                error = "empty prompt"
+            elif len(token_ids) >= self.engine.max_model_len:
+                error = (f"prompt length {len(token_ids)} exceeds "
+                         f"max_model_len {self.engine.max_model_len}")
+            elif peer is not None and peer.kv_cache_dtype != self._cache_kind():
+                error = (f"{decode_name} keeps another kind of cache "
+                         f"({peer.kv_cache_dtype or 'its own type'}) than "
+                         f"{self.name} ({self._cache_kind() or 'its own type'})")
+        if error is not None:
             if self.master_conn:
                 try:
                     await self.master_conn.notify("generations", gens=[dict(
                         service_request_id=service_request_id, token_ids=[],
-                        finished=True, finish_reason="abort",
-                        error=("empty prompt" if not token_ids else
-                               f"prompt length {len(token_ids)} exceeds "
-                               f"max_model_len {self.engine.max_model_len}"))])
+                        finished=True, finish_reason="abort", error=error)])
                 except Exception:
                     pass
             return

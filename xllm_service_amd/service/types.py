@@ -52,6 +52,7 @@ class InstanceMetaInfo:
     num_kv_blocks: int = 0
     block_size: int = 16
     model: str = ""
+    kv_cache_dtype: str = ""          # "fp8": pages of 8 bits; "": the model's type
     incarnation_id: int = 0
     register_ts_ms: int = field(default_factory=lambda: int(time.time() * 1000))
     # TTFT/TPOT profiling samples for the SLO predictor:
