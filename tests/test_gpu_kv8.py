@@ -128,6 +128,41 @@ def test_write_rows_at_any_address(offset):
     assert all(same(got.x[i], want.x[i]) for i in range(2))
 
 
+# a wave looks over one token, two, four or eight: from 375, 750 and 1500 tokens of 8
+# heads on, 250, 500 and 1000 of 12
+@pytest.mark.parametrize("heads,dim,tokens", [
+    (8, 128, 300), (8, 128, 400), (8, 128, 800), (8, 128, 1600), (8, 64, 1600),
+    (12, 64, 260), (12, 64, 600), (12, 64, 1100)])
+def test_write_by_windows(heads, dim, tokens):
+    """Uneven sequences that begin anywhere in a page: several runs to a window, runs
+    that begin in one and end in another, skipped tokens in and between them."""
+    g = torch.Generator().manual_seed(tokens + heads)
+    old, new = [], []
+    while sum(new) < tokens:
+        old.append(int(torch.randint(0, 40, (1,), generator=g)))
+        long = torch.rand(1, generator=g) < 0.2
+        new.append(int(torch.randint(1, 120 if long else 9, (1,), generator=g)))
+    lens = [a + b for a, b in zip(old, new)]
+    table, pages = layout(lens, 3, tokens)
+    cache = tuple(c.to(DEV) for c in ops.kv8_cache(pages, heads, dim))
+    want = Cache(pages, heads, dim)
+    for n, (a, b) in enumerate([([0] * len(old), old), (old, lens)]):
+        slots = []
+        for s in slots_of(table, a, b):
+            skip = torch.rand(2, generator=g)
+            if skip[0] < 0.08:
+                slots += [-1] * int(1 + 5 * skip[1])
+            slots.append(s)
+        k, v = (rows(len(slots), heads, dim, 2 * n + i, 3.0 ** n) for i in range(2))
+        gk, gv = part(k, heads, dim), part(v, heads, dim)
+        ops.reshape_and_cache_kv8(gk, gv, *cache, ints(slots, torch.long))
+        want.write(gk, gv, slots)
+        got = Cache(pages, heads, dim).load(*cache)
+        assert same(got.scale, want.scale), n
+        for i in range(2):
+            assert same(got.x[i], want.x[i]), (n, i)
+
+
 @pytest.mark.parametrize("heads,dim", [(3, 128), (2, 64)])
 def test_write_twice_to_a_slot(heads, dim):
     """The later one stays; the scale holds all of a page's new tokens, those that
@@ -556,6 +591,91 @@ def test_rows_without_keys():
     assert (got == 0).all()
     got = ops.paged_attn_prefill_kv8(q, *cache, none, ints(cu), ints([5, 9]), 0.1)
     assert (got == 0).all()
+
+
+def uneven(cache, want, seed):
+    """Pages' scales far apart."""
+    g = torch.Generator().manual_seed(seed)
+    by = torch.exp2(torch.randint(-3, 4, want.scale.shape, generator=g).double())
+    by[..., 0] = by[..., 0].clamp(max=1.0)
+    cache[2].mul_(by.float().to(DEV))
+    want.scale *= by
+
+
+def close_rows(got, q, want, table, old, new, scale, weights, at):
+    """Rows at[i] of every sequence, as those of a chunk that ends with them."""
+    start = 0
+    for i, (o, n) in enumerate(zip(old, new)):
+        for a, b in at:
+            a, b = min(a % n if a < 0 else a, n), min(b, n)
+            if a < b:
+                close(got[start + a:start + b], q[start + a:start + b], want,
+                      table[i:i + 1], [0, b - a], [o + b], scale, weights)
+        start += n
+
+
+# Pages' ids and scales are looked up for 16, 32 or 64 tiles at a time: sequences that
+# need a second and a third look, unsplit, in parts and by two groups of waves
+@pytest.mark.parametrize("heads,per,dim", [(8, 4, 128), (8, 8, 64), (8, 12, 64),
+                                           (8, 16, 128), (1, 4, 128), (1, 12, 128)])
+@pytest.mark.parametrize("scale", [0.02, 0.3])
+def test_decode_and_second_looks_at_tables(heads, per, dim, scale):
+    lens = [13 * i % 41 for i in range(100)]
+    lens[37], lens[71] = 9000, 4500
+    if heads == 1:                           # in parts of over 16 tiles a wave
+        lens = [90000, 3]
+    cache, want, table = filled(lens, heads, dim, 2)
+    uneven(cache, want, 1)
+    S = len(lens)
+    q = part(rows(S, heads * per, dim, 5), heads * per, dim)
+    got = ops.paged_attn_decode_kv8(q, *cache, table.to(DEV), ints(lens), scale)
+    close(got, q, want, table, list(range(S + 1)), lens, scale, 2.0 ** -15)
+
+
+FEW = [25] * 60
+SECOND = [(8, 4, 128, [200, 100], [4300, 10]), (8, 4, 64, [200, 100], [4300, 10]),
+          (8, 4, 128, FEW, [4400] + [3] * 59), (12, 1, 64, [1200] * 3 + [150],
+                                                [0, 0, 0, 8400]),
+          (8, 4, 128, [500], [17500]), (24, 8, 128, [600], [4100]),
+          (21, 8, 128, [300, 400], [100, 8300])]
+
+
+@pytest.mark.parametrize("heads,per,dim,new,old", SECOND)
+@pytest.mark.parametrize("scale", [0.02, 0.3])
+def test_prefill_and_second_looks_at_tables(heads, per, dim, new, old, scale):
+    lens = [a + b for a, b in zip(new, old)]
+    cache, want, table = filled(lens, heads, dim, 2)
+    uneven(cache, want, 1)
+    T = sum(new)
+    q = part(rows(T, heads * per, dim, 6), heads * per, dim)
+    cu = [sum(new[:i]) for i in range(len(new) + 1)]
+    got = ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints(cu), ints(lens),
+                                     scale)
+    close_rows(got, q, want, table, old, new, scale, 2.0 ** -8,
+               [(0, 9), (127, 133), (-7, 10 ** 6)])
+
+
+def test_entries_of_no_page_are_page_0():
+    """Whatever it holds, and only where keys are seen there."""
+    lens = [40, 25, 20]
+    cache, want, table = filled(lens, 2, 64, 4)
+    wild, zero = table.clone(), table.clone()
+    wild[0, 1], zero[0, 1] = 10 ** 6, 0
+    wild[1, 2], wild[2, 2] = -5, cache[2].shape[0]       # behind 32 keys
+    cache[1].view(torch.uint8)[0] = 0x7f
+    q = part(rows(9, 4, 64, 2), 4, 64)
+    cu = ints([0, 4, 6, 9])
+    for f, args in ((ops.paged_attn_decode_kv8, (q[:3],)),
+                    (ops.paged_attn_prefill_kv8, (q,))):
+        got = [f(*args, *cache, t.to(DEV), *((cu,) if len(args[0]) == 9 else ()),
+                 ints(lens), 0.1) for t in (wild, zero)]
+        bad = got[0].isnan()
+        assert torch.equal(bad, got[1].isnan())
+        assert torch.equal(got[0].nan_to_num(0.0), got[1].nan_to_num(0.0))
+        first = 1 if len(args[0]) == 3 else 4
+        assert bad[:first].all()
+        live = 0 in table[1, :2] or 0 in table[2, :2]
+        assert live or not bad[first:].any()
 
 
 def test_tables_that_end_before_their_sequence():
