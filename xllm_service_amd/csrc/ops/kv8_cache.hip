@@ -320,8 +320,10 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
         two = __builtin_elementwise_max(
             two, __builtin_bit_cast(u16x2, x[i][c] & 0x7fff7fffu));
     int big = __builtin_amdgcn_readlane(pf_scan<false>(max(two[0], two[1])), 63);
-    const bool odd = big >= 0x7f80;        // uniform: not all finite
-    if (__builtin_expect(odd, 0)) {
+    // rare, uniform: not all finite, or more tokens than places: those that later ones stand
+    // in the place of count for the scale too
+    const bool twice = r.n > __popc(r.have);
+    if (__builtin_expect(big >= 0x7f80 || twice, 0)) {
       big = 0;
 #pragma unroll
       for (int i = 0; i < NP; i++)
@@ -332,12 +334,8 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
             const int a = (int)(x[i][c] >> (16 * e)) & 0x7fff;
             big = max(big, a < 0x7f80 ? a : 0);
           }
-      big = __builtin_amdgcn_readlane(pf_scan<false>(big), 63);
-    }
-    // tokens that later ones stand in the place of count too
-    if (__builtin_expect(r.n > __popc(r.have), 0)) {
-      const int id = (int)((unsigned long)r.at / (unsigned)n_kv);
-      mask out = 0;
+      mask out = twice ? 0 : 1;
+      const int id = page_of(slot_at(r.from));
       for (int b = r.from; b < n_tokens && out == 0; b += 64) {
         const int p = page_of(slot_at(b + lane));
         out = __ballot(p >= 0 && p != id);
@@ -373,16 +371,6 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
                         __uint_as_float(b << 16) * by,
                         __uint_as_float(b & 0xffff0000u) * by);
       }
-      // 448 times the largest scale is past what fp32 and bf16 hold: what has become more
-      // than 240 of it is 240, half a step off at most as any other
-      if (__builtin_expect(__builtin_amdgcn_readfirstlane(now >= 0x1p120f), 0)) {
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          unsigned far = ((u[c] & 0x7f7f7f7fu) + 0x08080808u) & 0x80808080u & ~kv8_nan(u[c]);
-          far = (far >> 7) * 0x7fu;
-          u[c] = (u[c] & ~far) | (0x77777777u & far);
-        }
-      }
       if (!anew) {                         // uniform
         if (!keep) {
 #pragma unroll
@@ -404,6 +392,22 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
             make_uint4(u[0], u[1], u[2], u[3]);
     }
     if (lane == 0) kv_scale[2 * r.at + VAL] = now;
+    // rare, uniform: 448 times this scale is past what fp32 and bf16 hold. What has become
+    // more than 240 of it is 240, half a step off at most as any other. (Cut before it is
+    // written it kept registers that the rest wants: 7878 tokens 9.8 -> 10.2 us)
+    if (__builtin_expect(big > 0x7f70, 0)) {
+#pragma unroll 1
+      for (int i = 0; i < NP; i++) {
+        unsigned* at = reinterpret_cast<unsigned*>(to + place_of(i));
+#pragma unroll 1
+        for (int c = 0; c < 4; c++) {
+          const unsigned y = at[c];
+          unsigned far = ((y & 0x7f7f7f7fu) + 0x08080808u) & 0x80808080u & ~kv8_nan(y);
+          far = (far >> 7) * 0x7fu;
+          at[c] = (y & ~far) | (0x77777777u & far);
+        }
+      }
+    }
   };
   // one is loaded while the one before it is written
   Run a, b;
