@@ -13,6 +13,8 @@
 // applies it in the same instruction, and a page whose scale grows keeps its values
 // but for the subnormal ones, which are rounded once more. A finer scale would gain
 // e4m3 nothing: its step is relative to the value, 2^-4 at most, whatever the scale.
+// The largest scale is 2^120, of which finite values are 240 at most: 256 of it is not
+// finite in bf16 and 32 bits.
 #pragma once
 #include "mfma_rows.h"
 

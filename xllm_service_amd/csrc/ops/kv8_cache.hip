@@ -60,7 +60,7 @@ __global__ __launch_bounds__(SEQS) void kv8_plan_kernel(
         if (lo + step < n && at[lo + step] <= x) lo += step;
       return lo;
     };
-    // chunks of 256, every groups-th of them
+    // chunks of SEQS, every groups-th of them
     auto mine = [&](int from) {
       const int c = from / SEQS, ahead = (me - c % groups + groups) % groups;
       return (c + ahead) * SEQS + tid;
@@ -134,7 +134,7 @@ void launch_kv8_plan(int* tables, const int* seq_lens, const int* new_lens,
 // 11.5, 2000 of one 25 | 15.7 | 9.9 | 6.6 | 5.5, 300 4.9 | 4.4 | 4.4 | 4.3 | 4.3; a token each
 // of 1000 sequences 14.5 | 15.1 | 14.6 | 17.2 | 25, of 256 5.9 | 6.6 | 8.6 | 13.5 | 23.5, of 128
 // 4.4 | 5.3 | 7.7 | 12.5 | 22. One token: 3.7, a launch.
-//   7878 tokens are 48 MB: 11.0, 4.4 TB/s, of the 5.0 of a large copy. Before, by a wave to each
+//   7878 tokens are 48 MB: 11.2, 4.3 TB/s, of the 5.0 of a large copy. Before, by a wave to each
 // token and conversions of each value by itself, 47.4.
 typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
 
