@@ -155,7 +155,8 @@ XLLM_DEV void kv8_write_runs(const long* __restrict__ slots, const int n_tokens,
   };
   // Whether one of FAR tokens from t on has a slot, by loads that are waited for together:
   // padding is long and has none. Us, 64 at a time | so, 8 heads of 128: 10 tokens in front of
-  // padding to 8192 rows 33 | 11.4 (to 256, by 64 at a time, 5.5 | 6.4), to 65 k 238 | 52, to 2^20 5630 | 732.
+  // padding to 8192 rows 33 | 11.4, to 65 k 238 | 45, to 2^20 5630 | 739, but to 256 5.5 | 6.4:
+  // less than half as many are looked over 64 at a time.
   constexpr int FAR = 1024;
   auto any_from = [&](int t) {
     long s[FAR / 64];
