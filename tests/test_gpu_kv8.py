@@ -655,6 +655,34 @@ def test_prefill_and_second_looks_at_tables(heads, per, dim, new, old, scale):
                [(0, 9), (127, 133), (-7, 10 ** 6)])
 
 
+# many heads to one of the cache's, many sequences of few tokens, rows in front of the
+# first sequence and more behind the last one than there are in all
+OTHER = [(1, 32, 128, [40, 3], [500, 0], 60, 0, 3), (1, 71, 64, [33], [70], 300, 2, 1),
+         (2, 24, 128, [300], [90], 30, 0, 0), (1, 100, 128, [700], [60], 140, 0, 5),
+         (2, 4, 128, [i % 4 for i in range(300)], [7 * i % 101 for i in range(300)],
+          300, 1, 9),
+         (3, 1, 64, [i % 4 for i in range(300)], [7 * i % 101 for i in range(300)], 7,
+          0, 2),
+         (2, 4, 128, [20], [30], 4, 5, 700), (2, 4, 128, [20, 1], [1000, 30], 200, 5,
+                                              700),
+         (24, 8, 128, [600], [0], 140, 9, 800)]
+
+
+@pytest.mark.parametrize("heads,per,dim,new,old,width,front,behind", OTHER)
+def test_prefill_of_other_batches(heads, per, dim, new, old, width, front, behind):
+    lens = [n + o for n, o in zip(new, old)]
+    cache, want, table = filled(lens, heads, dim, 5, width=width)
+    H, T = heads * per, front + sum(new)
+    q = part(rows(T + behind, H, dim, 6), H, dim)
+    cu = [front + sum(new[:i]) for i in range(len(new) + 1)]
+    out = torch.full((T + behind, H, dim), 7.0, dtype=torch.bfloat16, device=DEV)
+    ops.paged_attn_prefill_kv8(q, *cache, table.to(DEV), ints(cu), ints(lens),
+                               dim ** -0.5, out=out)
+    close(out[front:T], q[front:T], want, table, [c - front for c in cu], lens,
+          dim ** -0.5, 2.0 ** -8)
+    assert (out[:front] == 7.0).all() and (out[T:] == 7.0).all()
+
+
 def test_entries_of_no_page_are_page_0():
     """Whatever it holds, and only where keys are seen there."""
     lens = [40, 25, 20]
